@@ -31,7 +31,7 @@ enum pp_status {
   PP_ENOSUPPORT = 3    /* valid request this build does not implement */
 };
 
-enum pp_dtype { PP_F16 = 0, PP_F32 = 1 };
+enum pp_dtype { PP_F16 = 0, PP_F32 = 1, PP_BF16 = 2 /* the serving operators' values only */ };
 
 /* Dual code layouts:
  *   PP_DUAL_I16_OFFSET -- native int16 = ((amp << 10) | phase) - 32768, the
@@ -47,7 +47,8 @@ const char* pp_last_error(void);
 const char* pp_version(void);
 
 /* sizeof of the ABI structs, for binding checks: out[0] = sizeof(pp_quad_proj),
- * out[1] = sizeof(pp_quad_item), out[2] = sizeof(pp_quad_seg), out[3] = sizeof(pp_dual_proj).
+ * out[1] = sizeof(pp_quad_item), out[2] = sizeof(pp_quad_seg), out[3] = sizeof(pp_dual_proj),
+ * out[4] = sizeof(pp_kv_cache).
  * Returns the number of values written. */
 int pp_abi_sizes(int64_t* out, int n);
 
@@ -734,6 +735,88 @@ int pp_dual_plug_table(const void* codes, int64_t n_codes, int code_layout, cons
                        int64_t group_size, int64_t chunk_size, const float* amp_lut, const uint32_t* plug_idx,
                        const void* plug_amp, int64_t plug_n, const int64_t* proj_pos0, const int32_t* proj_k,
                        int64_t n_projs, int64_t rows_per_task, uint32_t* ent, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Serving operators around the packed Linears: an 8-bit key/value cache, its */
+/* attention, log probabilities.  They have no counterpart in the reference.  */
+/* ------------------------------------------------------------------------ */
+
+/* Codes of a cache: int8 in -127..127, or float8 e4m3 (finite, no infinities). */
+enum pp_kv_codes { PP_KV_INT8 = 0, PP_KV_E4M3 = 1 };
+
+/*
+ * A paged cache: `pages` pages of `block` tokens (16, 32, 64 or 128) for `heads` heads of
+ * head_dim (64, 128, 192 or 256) values.  One byte a value: k is [page][head][token][d],
+ * v is [page][head][d][token], both dense at a 16-byte boundary; k_scale and v_scale are
+ * [page][head].  A value is code * scale.
+ *
+ * The sequences of a call: token t of sequence b lies in page table[b*table_ld + t / block]
+ * at place t % block; the call's tokens cu[b] .. cu[b+1]-1 (cu[0] taken as 0) are the last ones of
+ * sequence b's lengths[b] tokens.  cu may be null: one token each, tokens == batch.  table, lengths
+ * and cu are int32 in device memory; what they hold is held to its range on the device: a page
+ * outside [0, pages) or a token past the table's width is not written, reads zero and is seen by no
+ * row, and tokens past cu[batch] belong to no sequence.
+ */
+typedef struct pp_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int32_t heads, head_dim, block, codes;
+} pp_kv_cache;
+
+/*
+ * New keys and values into the cache: value (token, head, d) at k + token*k_st + head*k_sh + d
+ * (PP_F16 or PP_BF16; v alike).  For each page and head that gets tokens, k and v apart:
+ *   scale = max(old scale, max|x| / qmax, 2^-64),  qmax 127 or 448; the old scale counts if the
+ *           page holds earlier tokens of the sequence, whose codes become round(code * (old / scale))
+ *           where the scale grows;
+ *   code  = round(x * (1 / scale)) held to +-qmax, in float32, ties to even.
+ * A value that is not finite makes the page's scale not finite (and its codes 0), so that every row
+ * that sees the page is NaN, until the page begins anew.  A page that gets tokens belongs to one
+ * sequence of the call.
+ */
+int pp_kv_append(const pp_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                 int64_t v_sh, int dtype, int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
+                 const int32_t* lengths, const int32_t* cu, int64_t batch, void* stream);
+
+/*
+ * The values of a call's tokens, code * scale rounded once to `dtype` (PP_F16, PP_BF16, PP_F32), into
+ * dense (tokens, heads, head_dim) outputs at 16-byte boundaries.
+ */
+int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_t table_ld, int64_t table_width,
+               const int32_t* lengths, const int32_t* cu, int64_t batch, int64_t tokens, int dtype, void* k_out,
+               void* v_out, void* stream);
+
+/*
+ * Attention of a call's tokens to the cache.  Query head hq reads head hq / (q_heads / heads).  The row
+ * of the call's i-th token of sequence b has position p = lengths[b] - n_b + i and sees the keys of
+ * (p - window, p] (causal; window 0: of [0, p]), or all of [0, lengths[b]) (causal 0):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
+ * A row that sees no key gives zeros and lse -inf.  q is (tokens, q_heads, head_dim) with strides q_st,
+ * q_sh (PP_F16 or PP_BF16), out dense of the same type at a 16-byte boundary, lse null or (tokens,
+ * q_heads) float32.  The workspace (pp_kv_attention_workspace_size, 0: none) needs no initial values.
+ */
+int64_t pp_kv_attention_workspace_size(const pp_kv_cache* cache, int64_t table_width, int64_t batch, int64_t tokens,
+                                       int64_t q_heads);
+int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
+                    int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
+                    const int32_t* lengths, const int32_t* cu, int64_t batch, int causal, int64_t window, float scale,
+                    void* out, float* lse, void* workspace, int64_t workspace_size, void* stream);
+
+/*
+ * Log probabilities of rows of logits (row r at logits + r*l_st, V of them, PP_F16, PP_BF16 or PP_F32):
+ *   logprob[r*per_row + j] = x[tokens[r*t_st + j]] - lse   (NaN for a token outside [0, V)),
+ *   entropy[r] = lse - sum p x,   lse = log sum e^x,
+ *   top_ids / top_logprobs [r*top + j]: the `top` (at most 64) largest logits in order, equal ones by
+ *   the lower index, a NaN before all numbers.
+ * Logits of -inf count as probability 0; a row of nothing else, or with a NaN or +inf, gives NaN.
+ */
+int64_t pp_logprobs_workspace_size(int64_t rows, int64_t V, int64_t top);
+int pp_logprobs(const void* logits, int64_t l_st, int dtype, int64_t rows, int64_t V, const int64_t* tokens,
+                int64_t t_st, int64_t per_row, int64_t top, float* logprob, float* entropy, int64_t* top_ids,
+                float* top_logprobs, void* workspace, int64_t workspace_size, void* stream);
 
 #ifdef __cplusplus
 }

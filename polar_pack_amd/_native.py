@@ -14,7 +14,8 @@ import threading
 from .build import LIB
 
 PP_OK, PP_EINVAL, PP_EHIP, PP_ENOSUPPORT = 0, 1, 2, 3
-PP_F16, PP_F32 = 0, 1
+PP_F16, PP_F32, PP_BF16 = 0, 1, 2
+PP_KV_INT8, PP_KV_E4M3 = 0, 1
 PP_DUAL_I16_OFFSET, PP_DUAL_U16_BE = 0, 1
 PP_QUAD_NK, PP_QUAD_KN = 0, 1
 PP_GEMM_ROWS, PP_GEMM_KN, PP_GEMM_GENERIC = 1, 2, 3
@@ -50,6 +51,12 @@ class DualProj(C.Structure):
     """``pp_dual_proj`` (include/polar_pack.h)."""
     _fields_ = [("codes", vp), ("ldc", i64), ("pos0", i64), ("x", vp), ("x_sm", i64),
                 ("out", vp * 2), ("o_sm", i64), ("N", C.c_int32), ("K", C.c_int32)]
+
+
+class KVCache(C.Structure):
+    """``pp_kv_cache`` (include/polar_pack.h)."""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("pages", i64), ("heads", C.c_int32),
+                ("head_dim", C.c_int32), ("block", C.c_int32), ("codes", C.c_int32)]
 
 
 EXPORTS = {
@@ -133,6 +140,13 @@ EXPORTS = {
     "pp_quad_pack_norm": (i32, [vp, i32, i64, vp, vp, vp]),
     "pp_quad_pack_codes": (i32, [vp, i32, i64, f64, f64, vp, vp, vp]),
     "pp_dual_pack": (i32, [vp, vp, i32, i64, i64, i64, i32, f64, f64, vp, vp, vp]),
+    "pp_kv_append": (i32, [vp, vp, i64, i64, vp, i64, i64, i32, i64, vp, i64, i64, vp, vp, i64, vp]),
+    "pp_kv_read": (i32, [vp, vp, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp]),
+    "pp_kv_attention_workspace_size": (i64, [vp, i64, i64, i64, i64]),
+    "pp_kv_attention": (i32, [vp, vp, i64, i64, i64, i32, i64, vp, i64, i64, vp, vp, i64, i32, i64, C.c_float, vp, vp,
+                              vp, i64, vp]),
+    "pp_logprobs_workspace_size": (i64, [i64, i64, i64]),
+    "pp_logprobs": (i32, [vp, i64, i32, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp]),
     "pp_upload": (i32, [vp, vp, i64, vp]),
     "pp_upload_tables": (i32, [vp, vp, vp, i32, vp]),
 }
