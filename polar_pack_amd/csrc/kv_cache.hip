@@ -19,12 +19,13 @@ int kv_check_cache(const pp_kv_cache* c, KvCache* out) {
   return PP_OK;
 }
 
-int kv_check_seqs(const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths, const int32_t* cu,
+int kv_check_seqs(const KvCache& c, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths, const int32_t* cu,
                   int64_t batch, int64_t tokens, KvSeqs* out) {
   PP_REQUIRE(table && lengths, "kv: null block table or lengths");
   PP_REQUIRE(batch > 0 && batch <= (1 << 24), "kv: batch %lld not in 1..2^24", (long long)batch);
   PP_REQUIRE(tokens >= 0 && tokens <= (1 << 28), "kv: tokens %lld not in 0..2^28", (long long)tokens);
-  PP_REQUIRE(width > 0 && width <= (1 << 24), "kv: block table width %lld not in 1..2^24", (long long)width);
+  PP_REQUIRE(width > 0 && width <= (1 << 30) >> c.shift, "kv: a block table of %lld pages holds no or over 2^30 tokens",
+             (long long)width);
   PP_REQUIRE(ld >= width || batch == 1, "kv: block table rows of %lld overlap (stride %lld)", (long long)width,
              (long long)ld);
   PP_REQUIRE(cu != nullptr || tokens == batch, "kv: %lld tokens of %lld sequences need cu", (long long)tokens,
@@ -283,7 +284,7 @@ extern "C" int pp_kv_append(const pp_kv_cache* cache, const void* k, int64_t k_s
   AppendArgs A;
   int rc = kv_check_cache(cache, &A.C);
   if (rc) return rc;
-  rc = kv_check_seqs(table, table_ld, table_width, lengths, cu, batch, tokens, &A.S);
+  rc = kv_check_seqs(A.C, table, table_ld, table_width, lengths, cu, batch, tokens, &A.S);
   if (rc) return rc;
   PP_REQUIRE(dtype == PP_F16 || dtype == PP_BF16, "pp_kv_append: dtype %d is not PP_F16 or PP_BF16", dtype);
   if (tokens == 0) return PP_OK;
@@ -316,7 +317,7 @@ extern "C" int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_
   ReadArgs A;
   int rc = kv_check_cache(cache, &A.C);
   if (rc) return rc;
-  rc = kv_check_seqs(table, table_ld, table_width, lengths, cu, batch, tokens, &A.S);
+  rc = kv_check_seqs(A.C, table, table_ld, table_width, lengths, cu, batch, tokens, &A.S);
   if (rc) return rc;
   PP_REQUIRE(dtype == PP_F16 || dtype == PP_BF16 || dtype == PP_F32, "pp_kv_read: dtype %d", dtype);
   if (tokens == 0) return PP_OK;

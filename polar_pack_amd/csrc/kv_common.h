@@ -164,7 +164,7 @@ __device__ __forceinline__ void load8(const uint16_t* p, bool vec, float* x) {
 
 // Host side: the checks every entry point makes of a cache and its sequences.
 int kv_check_cache(const pp_kv_cache* c, KvCache* out);
-int kv_check_seqs(const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths, const int32_t* cu,
+int kv_check_seqs(const KvCache& c, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths, const int32_t* cu,
                   int64_t batch, int64_t tokens, KvSeqs* out);
 
 }  // namespace pp
