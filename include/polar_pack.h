@@ -796,14 +796,18 @@ int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_t table_ld,
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
  * A row that sees no key gives zeros and lse -inf.  q is (tokens, q_heads, head_dim) with strides q_st,
  * q_sh (PP_F16 or PP_BF16), out dense of the same type at a 16-byte boundary, lse null or (tokens,
- * q_heads) float32.  The workspace (pp_kv_attention_workspace_size, 0: none) needs no initial values.
+ * q_heads) float32.  The workspace (pp_kv_attention_workspace_size bytes, 0: none) needs no initial values;
+ * the counts (pp_kv_attention_counts_size bytes, 0: none) are zero on entry and left zero.
  */
-int64_t pp_kv_attention_workspace_size(const pp_kv_cache* cache, int64_t table_width, int64_t batch, int64_t tokens,
-                                       int64_t q_heads);
+int64_t pp_kv_attention_workspace_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
+                                       int64_t batch, int64_t tokens, int64_t q_heads);
+int64_t pp_kv_attention_counts_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
+                                    int64_t batch, int64_t tokens, int64_t q_heads);
 int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                     int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
                     const int32_t* lengths, const int32_t* cu, int64_t batch, int causal, int64_t window, float scale,
-                    void* out, float* lse, void* workspace, int64_t workspace_size, void* stream);
+                    void* out, float* lse, void* workspace, int64_t workspace_size, void* counts, int64_t counts_size,
+                    void* stream);
 
 /*
  * Log probabilities of rows of logits (row r at logits + r*l_st, V of them, PP_F16, PP_BF16 or PP_F32):

@@ -142,9 +142,10 @@ EXPORTS = {
     "pp_dual_pack": (i32, [vp, vp, i32, i64, i64, i64, i32, f64, f64, vp, vp, vp]),
     "pp_kv_append": (i32, [vp, vp, i64, i64, vp, i64, i64, i32, i64, vp, i64, i64, vp, vp, i64, vp]),
     "pp_kv_read": (i32, [vp, vp, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp]),
-    "pp_kv_attention_workspace_size": (i64, [vp, i64, i64, i64, i64]),
+    "pp_kv_attention_workspace_size": (i64, [i64] * 7),
+    "pp_kv_attention_counts_size": (i64, [i64] * 7),
     "pp_kv_attention": (i32, [vp, vp, i64, i64, i64, i32, i64, vp, i64, i64, vp, vp, i64, i32, i64, C.c_float, vp, vp,
-                              vp, i64, vp]),
+                              vp, i64, vp, i64, vp]),
     "pp_logprobs_workspace_size": (i64, [i64, i64, i64]),
     "pp_logprobs": (i32, [vp, i64, i32, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp]),
     "pp_upload": (i32, [vp, vp, i64, vp]),

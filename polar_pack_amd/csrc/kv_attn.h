@@ -16,8 +16,11 @@ struct AttnArgs {
   int64_t q_st, q_sh;
   uint16_t* out;
   float* lse;
-  float* parts;     // [token][query head][run][D + 4]: sums, maximum, sum of weights
-  int q_heads, group, window, causal, splits, q_vec;
+  float* parts;     // [head][workgroup][2][row][D + 4]: what a workgroup has of a row tile that it shares: sums of
+                    // values, maximum, sum of weights; 1: of the one that begins in it, 0: of one that began before
+  uint32_t* counts; // [head][workgroup]: parts that are done of the row tile that begins in it; 0 before and after
+  int q_heads, group, window, causal, q_vec;
+  int shares;       // workgroups a key/value head, 0: one a row tile
   float scale;      // of the scores, times log2(e)
 };
 
@@ -35,6 +38,15 @@ __device__ __forceinline__ void kv_visible(const AttnArgs& A, const RowTile& T, 
   hi = !real || pos < 0 ? 0 : A.causal && pos + 1 < T.lim ? (int)pos + 1 : T.lim;
 }
 
+// What the rows r0 .. r0 + R - 1 of a sequence see.
+__device__ __forceinline__ void kv_tile_range(const AttnArgs& A, int R, RowTile& T) {
+  const int i0 = T.r0 / A.group, last = min(T.rows, T.r0 + R) - 1;
+  int x;
+  kv_visible(A, T, i0, true, T.lo, x);
+  kv_visible(A, T, last / A.group, true, x, T.hi);
+  if (!A.causal && T.lim > 0) T.hi = T.lim;
+}
+
 // The tile of rows r0 .. r0 + R - 1; T.b and T.r0 are set.
 __device__ __forceinline__ bool kv_tile_fill(const AttnArgs& A, int R, RowTile& T) {
   const KvSeqs& S = A.S;
@@ -50,11 +62,7 @@ __device__ __forceinline__ bool kv_tile_fill(const AttnArgs& A, int R, RowTile& 
     const int64_t cap = (int64_t)S.width << A.C.shift;
     T.lim = len < 0 ? 0 : len < cap ? len : (int)cap;
   }
-  const int i0 = T.r0 / A.group, last = min(T.rows, T.r0 + R) - 1;
-  int x;
-  kv_visible(A, T, i0, true, T.lo, x);
-  kv_visible(A, T, last / A.group, true, x, T.hi);
-  if (!A.causal && T.lim > 0) T.hi = T.lim;
+  kv_tile_range(A, R, T);
   return true;
 }
 
@@ -73,22 +81,122 @@ __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, Ro
   return kv_tile_fill(A, R, T);
 }
 
-// The tile that holds query g of token `token`.
-__device__ __forceinline__ void kv_tile_of(const AttnArgs& A, int token, int g, int R, RowTile& T) {
-  T.b = A.S.cu == nullptr ? token : kv_find(A.S, token, 1, 1, 0);
-  T.r0 = ((token - kv_start(A.S, T.b)) * A.group + g) / R * R;
-  kv_tile_fill(A, R, T);
+// How the few-row kernel deals a call: its tiles of 64 keys, row tile after row tile, cut into equal
+// shares, one a workgroup, wherever that falls.  The lengths are on the device, so every workgroup
+// counts the tiles itself and finds where its share begins: thread t of 256 looks at sequences 4t .. 4t + 3,
+// then a sum and a scan over the workgroup.  A row tile that sees no key counts as one tile, the tokens
+// past cu[batch] are sequence `batch`.  Going on to a row tile costs a workgroup about as much as KV_TURN
+// tiles, so each begins with that many that hold no keys.
+constexpr int KV_TURN = 16;
+constexpr int KV_DEAL_BATCH = 1020;      // sequences that can be dealt; row tiles of more are not cut
+
+struct Deal {
+  int64_t at, end;    // tiles of the call that are this workgroup's and not done
+  int share;          // tiles a workgroup
+  int first, tiles;   // of each of the sequence's row tiles: key tile it begins at, tiles that hold keys
+  int into;           // tile of the row tile that `at` is, KV_TURN the first that holds keys
+};
+
+// What sequence b's row tiles have to read, and its rows.
+__device__ __forceinline__ int kv_sequence(const AttnArgs& A, int b, RowTile& T, int& first, int& tiles) {
+  const KvSeqs& S = A.S;
+  T.b = b;
+  const int len = S.lengths[b < S.batch ? b : 0];              // beside the offsets, not after them
+  T.s0 = kv_start(S, b);
+  const int n = kv_start(S, b + 1) - T.s0;
+  T.rows = n > 0 ? n * A.group : 0;
+  T.pos0 = T.lim = first = 0;
+  tiles = 1;
+  if (n <= 0) return 0;
+  if (b < S.batch) {
+    const int64_t cap = (int64_t)S.width << A.C.shift;
+    T.pos0 = len < 0 ? -n : len - n;
+    T.lim = len < 0 ? 0 : len < cap ? len : (int)cap;
+  }
+  int lo, hi, x;
+  kv_visible(A, T, 0, true, lo, x);
+  kv_visible(A, T, n - 1, true, x, hi);
+  if (!A.causal) hi = T.lim;
+  first = lo >> 6;
+  tiles = hi > lo ? ((hi + 63) >> 6) - first : 1;
+  return n;
 }
 
-// Runs of 64-key tiles: how many a row tile has, and the tiles [a, z) of run `split`.
-__device__ __forceinline__ int kv_runs(const AttnArgs& A, const RowTile& T, int split, int& a, int& z) {
-  const int first = T.lo >> 6, end = T.hi > T.lo ? (T.hi + 63) >> 6 : first;
-  const int tiles = end - first;
-  int run = (tiles + A.splits - 1) / A.splits;
-  run = run < 4 ? 4 : (run + 3) / 4 * 4;
-  a = first + split * run;
-  z = min(end, a + run);
-  return tiles > run ? (tiles + run - 1) / run : 1;
+__device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, Deal& U) {
+  __shared__ int64_t sums[4], from;
+  __shared__ int found[7];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t work[4], total = 0;
+  RowTile X[4];
+  int first[4], tiles[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int b = 4 * tid + k;
+    work[k] = 0;
+    if (b > A.S.batch) continue;
+    kv_sequence(A, b, X[k], first[k], tiles[k]);
+    work[k] = (int64_t)((X[k].rows + R - 1) / R) * (tiles[k] + KV_TURN);
+    total += work[k];
+  }
+  int64_t upto = total;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t v = __shfl_up((long long)upto, o, 64);
+    upto += lane >= o ? v : 0;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  const int64_t all = sums[0] + sums[1] + sums[2] + sums[3];
+  for (int w = 0; w < wave; ++w) upto += sums[w];
+  const int64_t share = (all + A.shares - 1) / A.shares;
+  U.share = (int)(share < 4 ? 4 : (share + 3) / 4 * 4);        // 4 wavefronts a workgroup
+  U.at = (int64_t)blockIdx.x * U.share;
+  U.end = U.at + U.share < all ? U.at + U.share : all;
+  if (U.at >= U.end) return false;
+  int64_t before = upto - total;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (U.at >= before && U.at < before + work[k]) {
+      found[0] = X[k].b;
+      found[1] = X[k].s0;
+      found[2] = X[k].rows;
+      found[3] = X[k].pos0;
+      found[4] = X[k].lim;
+      found[5] = first[k];
+      found[6] = tiles[k];
+      from = U.at - before;
+    }
+    before += work[k];
+  }
+  __syncthreads();
+  T.b = uniform(found[0]);
+  T.s0 = uniform(found[1]);
+  T.rows = uniform(found[2]);
+  T.pos0 = uniform(found[3]);
+  T.lim = uniform(found[4]);
+  U.first = uniform(found[5]);
+  U.tiles = uniform(found[6]);
+  const int64_t t = uniform64(from);
+  const int row_tile = (int)(t / (U.tiles + KV_TURN));
+  T.r0 = row_tile * R;
+  U.into = (int)(t - (int64_t)row_tile * (U.tiles + KV_TURN));
+  return true;
+}
+
+// On to the next row tile.
+__device__ __forceinline__ void kv_deal_next(const AttnArgs& A, int R, RowTile& T, Deal& U) {
+  U.into = 0;
+  T.r0 += R;
+  if (T.r0 < T.rows) return;
+  T.r0 = 0;
+  for (int b = T.b + 1; b <= A.S.batch; b += 64) {             // the next sequence that has tokens
+    const int e = b + (threadIdx.x & 63);
+    const uint64_t some = __ballot(e <= A.S.batch && kv_start(A.S, e + 1) > kv_start(A.S, e));
+    if (some) {
+      kv_sequence(A, b + __builtin_ctzll(some), T, U.first, U.tiles);
+      return;
+    }
+  }
 }
 
 __device__ __forceinline__ int lane_read(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
@@ -124,26 +232,41 @@ __device__ __forceinline__ void to_halves(u32x4 w, f16x8& a, f16x8& b) {
 
 // A row's query as the second operand of S^T = K Q^T: lane group g holds values 64 j + 16 g + 8 e + 0..7
 // as q[j][e], scaled by a power of two so that the largest lies in [2^13, 2^14): bf16 queries of any
-// size keep all their bits in fp16 (what is below 2^-37 of the largest loses some).  Returns the factor
-// of the row's sums, score scale and power of two; NaN for a row that is not finite.
-template <typename IO, int D>
-__device__ __forceinline__ float load_q(const AttnArgs& A, int token, int hq, int g, bool real, f16x8 (*q)[2]) {
-  float x[D / 64][2][8];
-  uint32_t top = 0;
+// size keep all their bits in fp16 (what is below 2^-37 of the largest loses some).  load_q issues the
+// loads, make_q returns the factor of the row's sums, score scale and power of two; NaN for a row that
+// is not finite.
+template <int D>
+__device__ __forceinline__ void load_q(const AttnArgs& A, int token, int hq, int g, bool real, u32x4 (*w)[2]) {
   const uint16_t* p = A.q + (int64_t)token * A.q_st + (int64_t)hq * A.q_sh + 16 * g;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (real) {
-        load8<IO>(p + 64 * j + 8 * e, A.q_vec, x[j][e]);
+      w[j][e] = u32x4{0, 0, 0, 0};
+      if (!real) continue;
+      const uint16_t* x = p + 64 * j + 8 * e;
+      if (A.q_vec) {
+        w[j][e] = *reinterpret_cast<const u32x4*>(x);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[j][e][k] = 0.f;
+        for (int k = 0; k < 4; ++k) w[j][e][k] = (uint32_t)x[2 * k] | (uint32_t)x[2 * k + 1] << 16;
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) top = max(top, mag(x[j][e][k]));
     }
+}
+
+template <typename IO, int D>
+__device__ __forceinline__ float make_q(const AttnArgs& A, const u32x4 (*w)[2], f16x8 (*q)[2]) {
+  float x[D / 64][2][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[j][e][k] = IO::get((uint16_t)(w[j][e][k / 2] >> (16 * (k & 1))));
+        top = max(top, mag(x[j][e][k]));
+      }
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   const float t = __uint_as_float(top);

@@ -7,6 +7,18 @@
 
 namespace pp {
 
+// (m, l, v) takes the part (mp, lp, w), both sums of e^(s - their maximum).
+template <int W>
+__device__ __forceinline__ void join_part(float& m, float& l, float* v, float mp, float lp, const float* w) {
+  const float mn = fmaxf(m, mp);
+  const float f = mp == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mp - mn);      // 1: nothing seen, 0 * 1
+  const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+  m = mn;
+  l = l * keep + lp * f;
+#pragma unroll
+  for (int k = 0; k < W; ++k) v[k] = v[k] * keep + w[k] * f;
+}
+
 // Few rows a sequence and head (single tokens, drafts).  A workgroup takes 16 * RT rows of one
 // sequence and key/value head and a run of 64-token tiles, dealt to its 4 wavefronts in turn; runs of
 // one row tile are joined by kv_attn_join_kernel.
@@ -19,32 +31,44 @@ namespace pp {
 // Scales stay out of the codes: ks multiplies a lane's scores, log2 vs is added to the exponent,
 // so that weights e^(s - m) vs are at most 2^14 in fp16 whatever the scales, and the sum of
 // e^(s - m) takes them times 1 / vs.
+template <int I>
+using Int = std::integral_constant<int, I>;
+
 template <int CODES, typename IO, int D, int RT, int NP>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(const AttnArgs A) {
-  constexpr int J = D / 64, DT = D / 16, R = 16 * RT;
+__global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A) {
+  constexpr int J = D / 64, DT = D / 16, R = 16 * RT, BUF = D * RT <= 256 ? 2 : 1;
   const KvCache& C = A.C;
   const KvSeqs& S = A.S;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), m16 = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % A.splits, h = blockIdx.y;
+  const int h = blockIdx.y;
   RowTile T;
-  if (!kv_row_tile(A, blockIdx.x / A.splits, R, T)) return;
-  int a, z;
-  const int ns = kv_runs(A, T, split, a, z);
-  if (split >= ns) return;
-  const int shift = C.shift, bs = C.block;
-
-  // this lane's rows: column m16 of row tile x
-  f16x8 q[RT][J][2];
-  float rf[RT];
-  int lo[RT], hi[RT];
-#pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    const int r = T.r0 + 16 * x + m16;
-    const bool real = r < T.rows;
-    const int i = real ? r / A.group : 0, gq = real ? r - i * A.group : 0;
-    kv_visible(A, T, i, real, lo[x], hi[x]);
-    rf[x] = load_q<IO, D>(A, T.s0 + i, h * A.group + gq, g, real, q[x]);
+  Deal U;
+  if (A.shares) {
+    if (!kv_deal(A, R, T, U)) return;
+  } else {
+    if (!kv_row_tile(A, blockIdx.x, R, T)) return;
+    U = Deal{0, 1, 1, T.lo >> 6, 1, 0};
   }
+  const int shift = C.shift, bs = C.block;
+  for (;; kv_deal_next(A, R, T, U)) {
+  int a = T.lo >> 6, z = T.hi > T.lo ? (T.hi + 63) >> 6 : 0, run = 0, runs = 1, owner = 0;
+  if (A.shares) {
+    const int64_t begin = U.at - U.into + KV_TURN;             // of its tiles that hold keys
+    const int left = U.tiles + KV_TURN - U.into;
+    const int take = U.end - U.at < left ? (int)(U.end - U.at) : left;
+    const int t0 = max(U.into - KV_TURN, 0), t1 = U.into + take - KV_TURN;
+    U.at += take;
+    if (t1 <= 0) return;                                       // the share ends before them
+    owner = (int)(begin / U.share);
+    runs = (int)((begin + U.tiles - 1) / U.share) - owner + 1;
+    run = blockIdx.x - owner;
+    kv_tile_range(A, R, T);
+    a = max(U.first + t0, T.lo >> 6);
+    z = min(U.first + t1, T.hi > T.lo ? (T.hi + 63) >> 6 : 0);
+  } else {
+    U.at = U.end;
+  }
+
   f32x4 o[RT][DT];
   float mx[RT], l[RT];
 #pragma unroll
@@ -59,15 +83,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
   // tile e / NP of the next 64 / NP tiles.
   const int32_t* table = S.table + (int64_t)T.b * S.ld;
   int ids = 0;
-  auto refill = [&](int tile) {
-    const int64_t at = (((int64_t)tile + 4 * (lane / NP)) * 64 >> shift) + lane % NP;
-    ids = at < S.width ? table[at] : -1;
-    ids = ids < C.pages ? ids : -1;
-  };
-  u32x4 kc[4][J], vc[DT];
-  float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
-  bool okv = false, ok_n = false;
-  int64_t vbase_n = 0;
   const int km = NP == 1 ? 0 : (16 * (m16 >> 2)) >> shift, vm = NP == 1 ? 0 : (16 * g) >> shift;   // page of the tile
   auto page_of = [&](int step, int which) {
     int p = lane_read(ids, (step % (64 / NP)) * NP);
@@ -78,37 +93,67 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
     }
     return p;
   };
-  auto load_k = [&](int tile, int step) {
-    int pk = page_of(step, km);
-    pk = pk < 0 ? 0 : pk;
-    const uint8_t* base = C.k + ((int64_t)pk * C.heads + h) * (bs * D);
+  // BUF tiles are on their way while one is worked on, each in registers of its own.  The loads of a
+  // tile past the last are made all the same, every lane's from the cache's first bytes: a branch
+  // around them would make the compiler wait for all loads at its end.
+  u32x4 kc[BUF][4][J], vc[BUF][DT];
+  float ks[BUF], vs[BUF];
+  int ok[BUF];
+  int64_t vat[BUF];
+  auto load_k = [&](auto buf, int tile, int step) {
+    constexpr int I = decltype(buf)::value;
+    const bool there = tile < z;
+    if (there && step % (64 / NP) == 0) {
+      const int64_t at = (((int64_t)tile + 4 * (lane / NP)) * 64 >> shift) + lane % NP;
+      ids = at < S.width ? table[at] : -1;
+      ids = ids < C.pages ? ids : -1;
+    }
+    const int pk = page_of(step, km), pv = page_of(step, vm);
+    const int64_t hk = (int64_t)((there & (pk >= 0)) ? pk : 0) * C.heads + (there ? h : 0);
     const int tok = (tile * 64 + 16 * (m16 >> 2)) & (bs - 1);
-    const int off = (tok + (m16 & 3)) * D + 16 * g;
+    const uint8_t* at = C.k + hk * (bs * D) + (there ? (tok + (m16 & 3)) * D + 16 * g : 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int j = 0; j < J; ++j) kc[t][j] = *reinterpret_cast<const u32x4*>(base + off + 4 * t * D + 64 * j);
-    const int pv = page_of(step, vm);
-    ok_n = pv >= 0;
-    const int64_t ph = (int64_t)(pv < 0 ? 0 : pv) * C.heads + h;
-    ks_n = C.ks[ph];
-    vs_n = C.vs[ph];
-    vbase_n = ph * (bs * D);
+      for (int j = 0; j < J; ++j) kc[I][t][j] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * j);
+    ok[I] = pv >= 0;
+    const int64_t ph = (int64_t)((there & (pv >= 0)) ? pv : 0) * C.heads + (there ? h : 0);
+    ks[I] = C.ks[ph];
+    vs[I] = C.vs[ph];
+    vat[I] = ph * (bs * D) + (there ? ((tile * 64 + 16 * g) & (bs - 1)) + m16 * bs : 0);
   };
-  auto load_v = [&](int tile) {
-    const uint8_t* base = C.v + vbase_n + ((tile * 64 + 16 * g) & (bs - 1)) + m16 * bs;
+  auto load_v = [&](auto buf) {
+    constexpr int I = decltype(buf)::value;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const u32x4*>(base + d * 16 * bs);
+    for (int d = 0; d < DT; ++d)
+      vc[I][d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(C.v + vat[I] + d * 16 * bs));
   };
 
+  // This lane's rows: column m16 of row tile x.
   int tile = a + wave, step = 0;
-  if (tile < z) {
-    refill(tile);
-    load_k(tile, 0);
-    load_v(tile);
+  u32x4 qw[RT][J][2];
+  int lo[RT], hi[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const int r = T.r0 + 16 * x + m16;
+    const bool real = r < T.rows;
+    const int i = real ? r / A.group : 0, gq = real ? r - i * A.group : 0;
+    kv_visible(A, T, i, real, lo[x], hi[x]);
+    load_q<D>(A, T.s0 + i, h * A.group + gq, g, real, qw[x]);
   }
-  for (; tile < z; tile += 4, ++step) {
-    ks = ks_n; vs = vs_n; okv = ok_n;
+  load_k(Int<0>(), tile, 0);
+  load_v(Int<0>());
+  if constexpr (BUF == 2) {
+    load_k(Int<BUF - 1>(), tile + 4, 1);
+    load_v(Int<BUF - 1>());
+  }
+  f16x8 q[RT][J][2];
+  float rf[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) rf[x] = make_q<IO, D>(A, qw[x], q[x]);
+
+  auto work = [&](auto buf) {
+    constexpr int I = decltype(buf)::value;
     f32x4 s[RT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -117,7 +162,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         f16x8 ka, kb;
-        to_halves<CODES>(kc[t][j], ka, kb);
+        to_halves<CODES>(kc[I][t][j], ka, kb);
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
           s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[x][j][0], s[x][t], 0, 0, 0);
@@ -125,29 +170,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
         }
       }
     }
-    const bool more = tile + 4 < z;
-    if (more) {
-      if ((step + 1) % (64 / NP) == 0) refill(tile + 4);
-      load_k(tile + 4, step + 1);
-    }
+    const bool okv = ok[I];
     // scores to weights
-    const bool vbad = mag(vs) >= 0x7f800000u;                    // the values are NaN, the sum of weights is not
-    const float vq = vbad ? 1.f : fmaxf(vs, KV_SCALE_MIN);
-    const float lv = __builtin_amdgcn_logf(vq), iv = 1.0f / vq;
+    const bool vbad = mag(vs[I]) >= 0x7f800000u;                 // the values are NaN, the sum of weights is not
+    const float vq = vbad ? 1.f : fmaxf(vs[I], KV_SCALE_MIN);
+    const float lv = __builtin_amdgcn_logf(vq), iv = 1.0f / vq, kscale = ks[I];
+    load_k(buf, tile + 4 * BUF, step + BUF);
     const int t0 = tile * 64 + 16 * g;
     f16x8 p[RT][2];
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
-      const float c = ks * rf[x];
-      const bool edge = __any(!okv || t0 < lo[x] || t0 + 16 > hi[x]);
+      const float c = kscale * rf[x];
+      const bool edge = __any(!okv | (t0 < lo[x]) | (t0 + 16 > hi[x]));
       float e[16], top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) e[4 * t + r] = s[x][t][r] * c + lv;
       if (edge) {
+        const int from = okv ? lo[x] - t0 : 16, to = hi[x] - t0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) e[k] = okv && t0 + k >= lo[x] && t0 + k < hi[x] ? e[k] : -INFINITY;
+        for (int k = 0; k < 16; ++k) e[k] = ((k >= from) & (k < to)) ? e[k] : -INFINITY;
       }
 #pragma unroll
       for (int k = 0; k < 16; ++k) top = fmaxf(top, e[k]);
@@ -170,9 +213,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
       }
       l[x] += sum * iv;
       if (__any(vbad)) {
+        const int from = (okv & vbad) ? lo[x] - t0 : 16, to = hi[x] - t0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (vbad && okv && t0 + k >= lo[x] && t0 + k < hi[x]) p[x][k / 8][k % 8] = (f16)NAN;
+        for (int k = 0; k < 16; ++k) p[x][k / 8][k % 8] = ((k >= from) & (k < to)) ? (f16)NAN : p[x][k / 8][k % 8];
       }
     }
     if (CODES == PP_KV_E4M3) {                   // codes past the length may be NaN
@@ -183,138 +226,179 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_split_kernel(co
           const int left = seen - 4 * w;
           const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) vc[d][w] &= keep;
+          for (int d = 0; d < DT; ++d) vc[I][d][w] &= keep;
         }
       }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       f16x8 va, vb;
-      to_halves<CODES>(vc[d], va, vb);
+      to_halves<CODES>(vc[I][d], va, vb);
 #pragma unroll
       for (int x = 0; x < RT; ++x) {
         o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[x][0], o[x][d], 0, 0, 0);
         o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, p[x][1], o[x][d], 0, 0, 0);
       }
     }
-    if (more) load_v(tile + 4);
+    load_v(buf);
+    tile += 4;
+    ++step;
+  };
+  while (tile < z) {
+    work(Int<0>());
+    if constexpr (BUF == 2) {
+      if (tile >= z) break;
+      work(Int<BUF - 1>());
+    }
   }
 
-  // The 4 wavefronts' sums meet in LDS: halves of them add the other half's, twice.
-  __shared__ float so[2][R][D + 4];
-  __shared__ float sm[2][R], sl[2][R];
-#pragma unroll
-  for (int x = 0; x < RT; ++x) l[x] = sum_groups(l[x]);
-#pragma unroll
-  for (int half = 2; half > 0; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-#pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        const int r = 16 * x + m16, w = wave - half;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&so[w][r][16 * d + 4 * g]) = o[x][d];
-        if (g == 0) { sm[w][r] = mx[x]; sl[w][r] = l[x]; }
-      }
-    }
-    __syncthreads();
-    if (wave < half) {
-#pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        const int r = 16 * x + m16;
-        const float mo = sm[wave][r], mn = fmaxf(mx[x], mo);
-        const float f = mx[x] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[x] - mn);
-        const float fo = mo == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mo - mn);
-        mx[x] = mn;
-        l[x] = l[x] * f + sl[wave][r] * fo;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[x][d] = o[x][d] * f + *reinterpret_cast<const f32x4*>(&so[wave][r][16 * d + 4 * g]) * fo;
-      }
-    }
-    __syncthreads();
-  }
-  if (wave != 0) return;
+  // The 4 wavefronts' sums meet in LDS; a thread then holds D / 16 neighbouring values of a row (of
+  // RT rows), of the run or, where the tile has several and this one is the last to end, of all.
+  constexpr int W = D / 16;
+  __shared__ float so[4][R][D + 4];
+  __shared__ float sm[4][R], sl[4][R];
+  __shared__ uint32_t done;
 #pragma unroll
   for (int x = 0; x < RT; ++x) {
-    const int r = T.r0 + 16 * x + m16;
+    const int r = 16 * x + m16;
+    l[x] = sum_groups(l[x]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&so[wave][r][16 * d + 4 * g]) = o[x][d];
+    if (g == 0) { sm[wave][r] = mx[x]; sl[wave][r] = l[x]; }
+  }
+  __syncthreads();
+  float v[RT][W], m[RT], sum[RT];
+  const int d0 = (threadIdx.x & 15) * W;
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const int r = 16 * x + (threadIdx.x >> 4);
+    m[x] = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    sum[x] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) v[x][k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = sm[w][r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][r] - m[x]);   // 0 * 1: nothing seen
+      sum[x] += sl[w][r] * f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[x][k] += so[w][r][d0 + k] * f;
+    }
+  }
+  bool last = true;
+  if (runs > 1) {
+    // A run's sums go to memory past the caches that other XCDs do not see (agent-scope stores) and
+    // are waited for before the tile's count goes up; the last run reads them all, in order, so that
+    // the result does not depend on which one is last.
+    // workgroup owner + i has part i; the owner's is its second
+    float* const part = A.parts + ((int64_t)h * A.shares + owner) * (2 * R) * (D + 4);
+    auto place = [&](int i) { return part + (int64_t)(i == 0 ? 1 : 2 * i) * R * (D + 4); };
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      const int r = 16 * x + (threadIdx.x >> 4);
+      if (T.r0 + r >= T.rows) continue;
+      float* p = place(run) + r * (D + 4);
+#pragma unroll
+      for (int k = 0; k < W; ++k) __hip_atomic_store(p + d0 + k, v[x][k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d0 == 0) {
+        __hip_atomic_store(p + D, m[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(p + D + 1, sum[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t* const count = A.counts + (int64_t)h * A.shares + owner;
+    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    last = done == (uint32_t)(runs - 1);
+    if (last) {
+    if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    // 16 threads a row and share of the runs: with few rows in the tile several shares a row
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      const int left = T.rows - T.r0 - 16 * x;
+      const int bits = left >= 9 ? 4 : left >= 5 ? 3 : left >= 3 ? 2 : left == 2 ? 1 : 0;
+      const int team = threadIdx.x >> 4, row = team & ((1 << bits) - 1), shares = 16 >> bits;
+      m[x] = -INFINITY;
+      sum[x] = 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[x][k] = 0.f;
+      if (row < left) {
+        constexpr int AHEAD = W <= 8 ? 8 : 4;
+        for (int i0 = team >> bits; i0 < runs; i0 += AHEAD * shares) {
+          f32x4 w[AHEAD][W / 4];
+          f32x2 ml[AHEAD];
+#pragma unroll
+          for (int u = 0; u < AHEAD; ++u) {
+            const int i = min(i0 + u * shares, runs - 1);
+            const float* e = place(i) + (16 * x + row) * (D + 4);
+            ml[u] = *reinterpret_cast<const f32x2*>(e + D);
+#pragma unroll
+            for (int k = 0; k < W / 4; ++k) w[u][k] = *reinterpret_cast<const f32x4*>(e + d0 + 4 * k);
+          }
+#pragma unroll
+          for (int u = 0; u < AHEAD; ++u)
+            if (i0 + u * shares < runs)
+              join_part<W>(m[x], sum[x], v[x], ml[u][0], ml[u][1], reinterpret_cast<const float*>(&w[u][0]));
+        }
+      }
+      __syncthreads();
+      float* mine = &so[0][team][0];
+#pragma unroll
+      for (int k = 0; k < W; ++k) mine[d0 + k] = v[x][k];
+      if (d0 == 0) { sm[0][team] = m[x]; sl[0][team] = sum[x]; }
+      __syncthreads();
+      for (int t = 1; t < shares; ++t) {
+        const int other = (row | t << bits) & 15;
+        if (team < 1 << bits) join_part<W>(m[x], sum[x], v[x], sm[0][other], sl[0][other], &so[0][other][d0]);
+      }
+    }
+    }
+  }
+  if (last) {
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const int r = T.r0 + 16 * x + (threadIdx.x >> 4);
     if (r >= T.rows) continue;
     const int i = r / A.group;
     const int64_t at = (int64_t)(T.s0 + i) * A.q_heads + h * A.group + (r - i * A.group);
-    if (ns == 1) {
-      const float inv = kv_inverse(l[x]);
+    const float inv = kv_inverse(sum[x]);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-        store4<IO>(A.out + at * D + 16 * d + 4 * g, o[x][d] * inv);
-      if (A.lse && g == 0) A.lse[at] = kv_lse(mx[x], l[x]);
-    } else {
-      float* part = A.parts + (at * A.splits + split) * (D + 4);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(part + 16 * d + 4 * g) = o[x][d];
-      if (g == 0) {
-        part[D] = mx[x];
-        part[D + 1] = l[x];
-      }
-    }
+    for (int k = 0; k < W; k += 4)
+      store4<IO>(A.out + at * D + d0 + k, f32x4{v[x][k] * inv, v[x][k + 1] * inv, v[x][k + 2] * inv, v[x][k + 3] * inv});
+    if (A.lse && d0 == 0) A.lse[at] = kv_lse(m[x], sum[x]);
   }
-}
-
-// One wavefront joins the runs of one row.
-template <typename IO, int D>
-__global__ __launch_bounds__(64) void kv_attn_join_kernel(const AttnArgs A, int R) {
-  const int64_t at = blockIdx.x;
-  const int token = (int)(at / A.q_heads), hq = (int)(at % A.q_heads), lane = threadIdx.x;
-  RowTile T;
-  kv_tile_of(A, token, hq % A.group, R, T);
-  int a, z;
-  const int ns = kv_runs(A, T, 0, a, z);
-  if (ns <= 1) return;
-  const float* part = A.parts + at * A.splits * (D + 4);
-  float m = -INFINITY;
-  for (int s = lane; s < ns; s += 64) m = fmaxf(m, part[s * (D + 4) + D]);
-  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  float l = 0.f, o[D / 64] = {};
-  for (int s = 0; s < ns; ++s) {
-    const float* p = part + s * (D + 4);
-    const float f = p[D] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p[D] - m);
-    l += p[D + 1] * f;
-#pragma unroll
-    for (int x = 0; x < D / 64; ++x) o[x] += p[64 * x + lane] * f;
   }
-  const float inv = kv_inverse(l);
-#pragma unroll
-  for (int x = 0; x < D / 64; ++x) A.out[at * D + 64 * x + lane] = IO::put(o[x] * inv);
-  if (A.lse && lane == 0) A.lse[at] = kv_lse(m, l);
+  if (U.at >= U.end) return;
+  __syncthreads();                       // the sums in LDS are read
+  }
 }
 
 struct AttnPlan {
   int rt;
-  int64_t splits, bytes;
+  int64_t shares, grid, bytes, counts;
 };
 
-static AttnPlan attn_plan(const pp_kv_cache* c, int64_t width, int64_t batch, int64_t tokens, int64_t q_heads) {
-  const int64_t rows = (tokens * (q_heads / c->heads) + batch - 1) / batch;      // a sequence and head, on average
+// The row tile by the mean rows a sequence and head; a workgroup a CU.
+static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
+                          int64_t q_heads) {
+  const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch;
   AttnPlan P;
   P.rt = rows > 16 ? 2 : 1;
-  const int64_t items = batch * ((rows + 16 * P.rt - 1) / (16 * P.rt)) * c->heads;
-  // two workgroups a CU; a run is at least 4 tiles
-  const int64_t most = (width * c->block + 255) / 256;
-  int64_t s = (2 * (int64_t)device_cu_count() + items - 1) / items;
-  if (s > most) s = most;
-  if (s < 1) s = 1;
-  P.splits = s;
-  P.bytes = s > 1 ? tokens * q_heads * s * (c->head_dim + 4) * 4 : 0;
+  const int64_t R = 16 * P.rt, row_tiles = tokens * group / R + batch + 1;
+  P.shares = (device_cu_count() + heads - 1) / heads;
+  const int64_t most = row_tiles * ((width * block + 255) / 256 + 1);       // of 4 tiles each
+  if (P.shares > most) P.shares = most;
+  if (batch > KV_DEAL_BATCH) P.shares = 0;
+  P.grid = P.shares ? P.shares : row_tiles;
+  P.bytes = heads * P.shares * 2 * R * (D + 4) * 4;
+  P.counts = heads * P.shares * 4;
   return P;
-}
-
-// Row tiles of R rows that the call may have: those of the sequences begin at floor(rows before / R) + b.
-static int64_t attn_items(const AttnArgs& A, int R) {
-  return A.S.cu ? (int64_t)A.S.tokens * A.group / R + A.S.batch + 1
-                : (int64_t)A.S.batch * ((A.group + R - 1) / R);
 }
 
 template <int CODES, typename IO, int D>
 static int attn_launch(const AttnArgs& A, const AttnPlan& P, hipStream_t st) {
-  const dim3 grid((unsigned)(attn_items(A, 16 * P.rt) * P.splits), (unsigned)A.C.heads);
+  const dim3 grid((unsigned)P.grid, (unsigned)A.C.heads);
   auto pick = [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
     auto kern = A.C.block >= 64 ? kv_attn_split_kernel<CODES, IO, D, RT, 1>
@@ -324,11 +408,6 @@ static int attn_launch(const AttnArgs& A, const AttnPlan& P, hipStream_t st) {
   if (P.rt == 1) pick(std::integral_constant<int, 1>());
   else pick(std::integral_constant<int, 2>());
   PP_LAUNCH_CHECK();
-  if (P.splits > 1) {
-    hipLaunchKernelGGL((kv_attn_join_kernel<IO, D>), dim3((unsigned)((int64_t)A.S.tokens * A.q_heads)), dim3(64), 0, st,
-                       A, 16 * P.rt);
-    PP_LAUNCH_CHECK();
-  }
   return PP_OK;
 }
 
@@ -346,18 +425,30 @@ static int attn_width(const AttnArgs& A, const AttnPlan& P, int D, hipStream_t s
 
 using namespace pp;
 
-extern "C" int64_t pp_kv_attention_workspace_size(const pp_kv_cache* cache, int64_t table_width, int64_t batch,
-                                                  int64_t tokens, int64_t q_heads) {
-  KvCache c;
-  if (kv_check_cache(cache, &c) || table_width <= 0 || batch <= 0 || tokens <= 0 || q_heads < cache->heads) return 0;
-  return attn_plan(cache, table_width, batch, tokens, q_heads).bytes;
+static bool attn_sizes(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
+                       int64_t q_heads, AttnPlan* P) {
+  if (heads <= 0 || D <= 0 || block <= 0 || width <= 0 || batch <= 0 || tokens <= 0 || q_heads < heads) return false;
+  *P = attn_plan(heads, D, block, width, batch, tokens, q_heads);
+  return true;
+}
+
+extern "C" int64_t pp_kv_attention_workspace_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
+                                                  int64_t batch, int64_t tokens, int64_t q_heads) {
+  AttnPlan P;
+  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, &P) ? P.bytes : 0;
+}
+
+extern "C" int64_t pp_kv_attention_counts_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
+                                               int64_t batch, int64_t tokens, int64_t q_heads) {
+  AttnPlan P;
+  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, &P) ? P.counts : 0;
 }
 
 extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads,
                                int dtype, int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
                                const int32_t* lengths, const int32_t* cu, int64_t batch, int causal, int64_t window,
                                float scale, void* out, float* lse, void* workspace, int64_t workspace_size,
-                               void* stream) {
+                               void* counts, int64_t counts_size, void* stream) {
   AttnArgs A;
   int rc = kv_check_cache(cache, &A.C);
   if (rc) return rc;
@@ -371,9 +462,11 @@ extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t 
   if (tokens == 0) return PP_OK;
   PP_REQUIRE(q && out, "pp_kv_attention: null queries or output");
   PP_REQUIRE(aligned(q, 2) && aligned(out, 16), "pp_kv_attention: queries or output are not aligned");
-  const AttnPlan P = attn_plan(cache, table_width, batch, tokens, q_heads);
+  const AttnPlan P = attn_plan(A.C.heads, cache->head_dim, A.C.block, table_width, batch, tokens, q_heads);
   PP_REQUIRE(P.bytes == 0 || (workspace && workspace_size >= P.bytes && aligned(workspace, 16)),
              "pp_kv_attention: workspace of %lld bytes at a 16-byte boundary needed", (long long)P.bytes);
+  PP_REQUIRE(P.counts == 0 || (counts && counts_size >= P.counts && aligned(counts, 4)),
+             "pp_kv_attention: %lld bytes of counts, zero, needed", (long long)P.counts);
   A.q = (const uint16_t*)q;
   A.q_st = q_st; A.q_sh = q_sh;
   A.q_vec = aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0;
@@ -384,8 +477,9 @@ extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t 
   A.group = (int)q_heads / A.C.heads;
   A.window = (int)(window < INT32_MAX ? window : 0);
   A.causal = causal;
-  A.splits = (int)P.splits;
-  PP_REQUIRE(attn_items(A, 16 * P.rt) * P.splits <= INT32_MAX, "pp_kv_attention: too many rows");
+  A.shares = (int)P.shares;
+  A.counts = (uint32_t*)counts;
+  PP_REQUIRE(P.grid <= INT32_MAX, "pp_kv_attention: too many rows");
   A.scale = scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
   const int D = cache->head_dim;

@@ -182,11 +182,16 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
     with torch.cuda.device(dev):
         out = torch.empty((n, heads, cache.head_dim), dtype=q.dtype, device=dev)
         lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
-        L = nat.lib()
-        size = L.pp_kv_attention_workspace_size(cache._ref, call[2], call[5], n, heads)
+        shape = (dev.index, cache.heads, cache.head_dim, cache.block, call[2], call[5], n, heads)
+        size = nat.sized("pp_kv_attention_workspace_size", *shape)
+        n_counts = nat.sized("pp_kv_attention_counts_size", *shape)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        nat.check(L.pp_kv_attention(cache._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _VALUES[q.dtype], n,
-                                    *call, int(causal), int(window), scale, out.data_ptr(),
-                                    lse.data_ptr() if return_lse else None, ws.data_ptr() if size else None, size,
-                                    nat.raw_stream(dev)), "pp_kv_attention")
+        counts, key = nat.zero_workspace(dev, n_counts)
+        rc = nat.lib().pp_kv_attention(cache._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _VALUES[q.dtype], n,
+                                       *call, int(causal), int(window), scale, out.data_ptr(),
+                                       lse.data_ptr() if return_lse else None, ws.data_ptr() if size else None, size,
+                                       counts.data_ptr() if n_counts else None, n_counts, nat.raw_stream(dev))
+        if rc:
+            nat.drop_workspace(key)
+        nat.check(rc, "pp_kv_attention")
     return (out, lse) if return_lse else out
