@@ -9,6 +9,11 @@ namespace pp {
 // largest.
 constexpr float KV_P_LOG2 = 14.f;
 
+// A row tile of many rows whose keys several workgroups share: the parts, and the rows.
+struct ManyPart {
+  int runs, s0, r0, rows;
+};
+
 struct AttnArgs {
   KvCache C;
   KvSeqs S;
@@ -18,6 +23,7 @@ struct AttnArgs {
   float* lse;
   float* parts;     // [head][workgroup][2][row][D + 4]: what a workgroup has of a row tile that it shares: sums of
                     // values, maximum, sum of weights; 1: of the one that begins in it, 0: of one that began before
+  ManyPart* desc;   // [head][workgroup] (many rows): the shared row tile that begins in it, runs 0: none
   uint32_t* counts; // [head][workgroup]: parts that are done of the row tile that begins in it; 0 before and after
   int q_heads, group, window, causal, q_vec;
   int shares;       // workgroups a key/value head, 0: one a row tile
@@ -215,6 +221,16 @@ __device__ __forceinline__ float sum_groups(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Over the lanes l, l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // 16 codes as two operands of 8 halves.
 template <int CODES>
 __device__ __forceinline__ void to_halves(u32x4 w, f16x8& a, f16x8& b) {
@@ -254,31 +270,59 @@ __device__ __forceinline__ void load_q(const AttnArgs& A, int token, int hq, int
     }
 }
 
-template <typename IO, int D>
-__device__ __forceinline__ float make_q(const AttnArgs& A, const u32x4 (*w)[2], f16x8 (*q)[2]) {
-  float x[D / 64][2][8];
+// PARTS 16-byte pieces of a row as halves; the row's other pieces are in the lanes lane ^ FROM, lane ^ 2 FROM .. .
+template <typename IO, int PARTS, int FROM>
+__device__ __forceinline__ float scale_q(const AttnArgs& A, const u32x4* w, f16x8* q) {
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j)
+  for (int j = 0; j < PARTS; ++j)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int k = 0; k < 8; ++k) top = max(top, mag(IO::get((uint16_t)(w[j][k / 2] >> (16 * (k & 1))))));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[j][e][k] = IO::get((uint16_t)(w[j][e][k / 2] >> (16 * (k & 1))));
-        top = max(top, mag(x[j][e][k]));
-      }
-#pragma unroll
-  for (int o = 16; o < 64; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-  const float t = __uint_as_float(top);
+  for (int o = FROM; o < 64; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   const bool finite = top < 0x7f800000u;
-  const int ex = top == 0 || !finite ? 0 : 14 - __builtin_amdgcn_frexp_expf(t);
+  const int ex = top == 0 || !finite ? 0 : 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j)
+  for (int j = 0; j < PARTS; ++j)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) q[j][e][k] = (f16)ldexpf(x[j][e][k], ex);
+    for (int k = 0; k < 8; ++k) q[j][k] = (f16)ldexpf(IO::get((uint16_t)(w[j][k / 2] >> (16 * (k & 1)))), ex);
   return finite ? ldexpf(A.scale, -ex) : NAN;
+}
+
+template <typename IO, int D>
+__device__ __forceinline__ float make_q(const AttnArgs& A, const u32x4 (*w)[2], f16x8 (*q)[2]) {
+  return scale_q<IO, D / 32, 16>(A, &w[0][0], &q[0][0]);
+}
+
+// The same for 32 rows a product: lane half hh holds values 16 c + 8 hh + 0..7 as q[c].
+template <typename IO, int D>
+__device__ __forceinline__ float many_q(const AttnArgs& A, int token, int hq, int hh, bool real, f16x8* q) {
+  const uint16_t* p = A.q + (int64_t)token * A.q_st + (int64_t)hq * A.q_sh + 8 * hh;
+  u32x4 w[D / 16];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    w[c] = u32x4{0, 0, 0, 0};
+    if (!real) continue;
+    if (A.q_vec) {
+      w[c] = *reinterpret_cast<const u32x4*>(p + 16 * c);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[c][k] = (uint32_t)p[16 * c + 2 * k] | (uint32_t)p[16 * c + 2 * k + 1] << 16;
+    }
+  }
+  return scale_q<IO, D / 16, 32>(A, w, q);
+}
+
+// (m, l, v) takes the part (mp, lp, w), both sums of e^(s - their maximum).
+template <int W>
+__device__ __forceinline__ void join_part(float& m, float& l, float* v, float mp, float lp, const float* w) {
+  const float mn = fmaxf(m, mp);
+  const float f = mp == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mp - mn);      // 1: nothing seen, 0 * 1
+  const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+  m = mn;
+  l = l * keep + lp * f;
+#pragma unroll
+  for (int k = 0; k < W; ++k) v[k] = v[k] * keep + w[k] * f;
 }
 
 // 1 / l, and 0 for a row that saw nothing; a NaN stays.
@@ -294,5 +338,13 @@ __device__ __forceinline__ void store4(uint16_t* p, f32x4 v) {
   w[1] = (uint32_t)IO::put(v[2]) | (uint32_t)IO::put(v[3]) << 16;
   *reinterpret_cast<u32x2*>(p) = w;
 }
+
+struct AttnPlan {
+  int64_t rows;       // rows of a row tile: 16, 32 (few rows a sequence and head), 128 or 256 (many)
+  int64_t shares, grid, bytes, counts;
+};
+
+// Prompts (kv_attn_many.hip).
+int kv_attn_many(const AttnArgs& A, const AttnPlan& P, int D, int codes, int dtype, hipStream_t st);
 
 }  // namespace pp

@@ -7,18 +7,6 @@
 
 namespace pp {
 
-// (m, l, v) takes the part (mp, lp, w), both sums of e^(s - their maximum).
-template <int W>
-__device__ __forceinline__ void join_part(float& m, float& l, float* v, float mp, float lp, const float* w) {
-  const float mn = fmaxf(m, mp);
-  const float f = mp == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mp - mn);      // 1: nothing seen, 0 * 1
-  const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-  m = mn;
-  l = l * keep + lp * f;
-#pragma unroll
-  for (int k = 0; k < W; ++k) v[k] = v[k] * keep + w[k] * f;
-}
-
 // Few rows a sequence and head (single tokens, drafts).  A workgroup takes 16 * RT rows of one
 // sequence and key/value head and a run of 64-token tiles, dealt to its 4 wavefronts in turn; runs of
 // one row tile are joined by kv_attn_join_kernel.
@@ -374,25 +362,20 @@ __global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A)
   }
 }
 
-struct AttnPlan {
-  int rt;
-  int64_t shares, grid, bytes, counts;
-};
-
 // The row tile by the mean rows a sequence and head; a workgroup a CU.
 static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
                           int64_t q_heads) {
-  const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch;
+  const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch, cus = device_cu_count();
   AttnPlan P;
-  P.rt = rows > 16 ? 2 : 1;
-  const int64_t R = 16 * P.rt, row_tiles = tokens * group / R + batch + 1;
-  P.shares = (device_cu_count() + heads - 1) / heads;
+  P.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 || D > 128 ? 128 : 256;
+  const int64_t row_tiles = tokens * group / P.rows + batch + 1;
+  P.shares = (cus + heads - 1) / heads;
   const int64_t most = row_tiles * ((width * block + 255) / 256 + 1);       // of 4 tiles each
   if (P.shares > most) P.shares = most;
-  if (batch > KV_DEAL_BATCH) P.shares = 0;
+  if (batch > KV_DEAL_BATCH || (P.rows > 32 && tokens * q_heads / P.rows >= 2 * cus)) P.shares = 0;
   P.grid = P.shares ? P.shares : row_tiles;
-  P.bytes = heads * P.shares * 2 * R * (D + 4) * 4;
-  P.counts = heads * P.shares * 4;
+  P.bytes = heads * P.shares * (2 * P.rows * (D + 4) * 4 + (int64_t)sizeof(ManyPart));
+  P.counts = P.rows <= 32 ? heads * P.shares * 4 : 0;
   return P;
 }
 
@@ -405,7 +388,7 @@ static int attn_launch(const AttnArgs& A, const AttnPlan& P, hipStream_t st) {
                 : A.C.block == 32 ? kv_attn_split_kernel<CODES, IO, D, RT, 2> : kv_attn_split_kernel<CODES, IO, D, RT, 4>;
     hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, A);
   };
-  if (P.rt == 1) pick(std::integral_constant<int, 1>());
+  if (P.rows == 16) pick(std::integral_constant<int, 1>());
   else pick(std::integral_constant<int, 2>());
   PP_LAUNCH_CHECK();
   return PP_OK;
@@ -478,11 +461,13 @@ extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t 
   A.window = (int)(window < INT32_MAX ? window : 0);
   A.causal = causal;
   A.shares = (int)P.shares;
+  A.desc = P.shares ? (ManyPart*)(A.parts + A.C.heads * P.shares * 2 * P.rows * (cache->head_dim + 4)) : nullptr;
   A.counts = (uint32_t*)counts;
   PP_REQUIRE(P.grid <= INT32_MAX, "pp_kv_attention: too many rows");
   A.scale = scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
   const int D = cache->head_dim;
+  if (P.rows > 32) return kv_attn_many(A, P, D, cache->codes, dtype, st);
   if (cache->codes == PP_KV_INT8)
     return dtype == PP_F16 ? attn_width<PP_KV_INT8, IoF16>(A, P, D, st) : attn_width<PP_KV_INT8, IoBf16>(A, P, D, st);
   return dtype == PP_F16 ? attn_width<PP_KV_E4M3, IoF16>(A, P, D, st) : attn_width<PP_KV_E4M3, IoBf16>(A, P, D, st);
