@@ -89,8 +89,8 @@ __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, Ro
 
 // How the few-row kernel deals a call: its tiles of 64 keys, row tile after row tile, cut into equal
 // shares, one a workgroup, wherever that falls.  The lengths are on the device, so every workgroup
-// counts the tiles itself and finds where its share begins: thread t of 256 looks at sequences 4t .. 4t + 3,
-// then a sum and a scan over the workgroup.  A row tile that sees no key counts as one tile, the tokens
+// counts the tiles itself and finds where its share begins: thread t of 256 looks at sequences 4t .. 4t + 3
+// (of 512 at 2t, 2t + 1), then a sum and a scan over the workgroup.  A row tile that sees no key counts as one tile, the tokens
 // past cu[batch] are sequence `batch`.  Going on to a row tile costs a workgroup about as much as KV_TURN
 // tiles, so each begins with that many that hold no keys.
 constexpr int KV_TURN = 16;
@@ -128,16 +128,18 @@ __device__ __forceinline__ int kv_sequence(const AttnArgs& A, int b, RowTile& T,
   return n;
 }
 
+template <int THREADS>
 __device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, Deal& U) {
-  __shared__ int64_t sums[4], from;
+  __shared__ int64_t sums[THREADS / 64], from;
   __shared__ int found[7];
+  constexpr int PER = 1024 / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t work[4], total = 0;
-  RowTile X[4];
-  int first[4], tiles[4];
+  int64_t work[PER], total = 0;
+  RowTile X[PER];
+  int first[PER], tiles[PER];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int b = 4 * tid + k;
+  for (int k = 0; k < PER; ++k) {
+    const int b = PER * tid + k;
     work[k] = 0;
     if (b > A.S.batch) continue;
     kv_sequence(A, b, X[k], first[k], tiles[k]);
@@ -152,7 +154,9 @@ __device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, De
   }
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
-  const int64_t all = sums[0] + sums[1] + sums[2] + sums[3];
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) all += sums[w];
   for (int w = 0; w < wave; ++w) upto += sums[w];
   const int64_t share = (all + A.shares - 1) / A.shares;
   U.share = (int)(share < 4 ? 4 : (share + 3) / 4 * 4);        // 4 wavefronts a workgroup
@@ -161,7 +165,7 @@ __device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, De
   if (U.at >= U.end) return false;
   int64_t before = upto - total;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < PER; ++k) {
     if (U.at >= before && U.at < before + work[k]) {
       found[0] = X[k].b;
       found[1] = X[k].s0;

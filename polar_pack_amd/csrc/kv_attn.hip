@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A)
   RowTile T;
   Deal U;
   if (A.shares) {
-    if (!kv_deal(A, R, T, U)) return;
+    if (!kv_deal<256>(A, R, T, U)) return;
   } else {
     if (!kv_row_tile(A, blockIdx.x, R, T)) return;
     U = Deal{0, 1, 1, T.lo >> 6, 1, 0};

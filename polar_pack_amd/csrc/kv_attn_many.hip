@@ -1,8 +1,8 @@
 // Attention of many rows a sequence and head (prompts, pieces of prompts) to the 8-bit cache.
 //
-// A workgroup of 4 wavefronts takes 128 NQ rows of one sequence and key/value head, a wavefront 32 NQ
-// of them, and walks the keys in tiles of 64.  The codes of a tile become fp16 once, on their way
-// into LDS, for all four wavefronts; both products run on v_mfma_f32_32x32x16_f16.
+// A workgroup of 4 or 8 wavefronts takes 32 rows a wavefront of one sequence and key/value head and
+// walks the keys in tiles of 64.  The codes of a tile become fp16 once, on their way
+// into LDS, for all wavefronts; both products run on v_mfma_f32_32x32x16_f16.
 //
 // S^T = K Q^T leaves a lane 16 scores of one row (column lane % 32) for each 32 keys.  Which key is
 // which row of the product is free: row m takes the key whose bits 2 and 3 are those of m swapped, so
@@ -13,15 +13,18 @@
 
 namespace pp {
 
+constexpr float KV_NONE = -1e30f, KV_NEAR = 12.f, KV_FAR = 15.9f;
+
 // 16-byte chunk c of row r: rows of a multiple of 256 bytes by r % 16, of an odd multiple of 128 by r / 2 % 8.
 template <int BYTES>
 __device__ __forceinline__ int swizzled(int r, int c) {
   return BYTES % 256 == 0 ? r * BYTES + 16 * (c ^ (r & 15)) : r * BYTES + 16 * (c ^ ((r >> 1) & 7));
 }
 
-template <int CODES, typename IO, int D, int NQ, int NP>
-__global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) {
-  constexpr int KS = D / 16, DT = D / 32, R = 128 * NQ, CH = D / 64;   // chunks of 16 codes a thread stages
+template <int CODES, typename IO, int D, int WAVES, int NP>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(const AttnArgs A) {
+  constexpr int KS = D / 16, DT = D / 32, R = 32 * WAVES, THREADS = 64 * WAVES;
+  constexpr int CH = 4 * D < THREADS ? 1 : 4 * D / THREADS;            // chunks of 16 codes of K and of V a thread stages
   constexpr int KB = 64 * D * 2;                                       // bytes of a tile of K or V
   __shared__ __align__(16) uint8_t lds[2][2 * KB];
   const KvCache& C = A.C;
@@ -33,7 +36,7 @@ __global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) 
   ManyPart* const desc = A.desc ? A.desc + (int64_t)h * A.shares + blockIdx.x : nullptr;
   if (A.shares) {
     if (tid == 0) desc->runs = 0;
-    if (!kv_deal(A, R, T, U)) return;
+    if (!kv_deal<THREADS>(A, R, T, U)) return;
   } else {
     // the last row tiles first: they see the most keys
     if (!kv_row_tile(A, gridDim.x - 1 - blockIdx.x, R, T)) return;
@@ -59,31 +62,24 @@ __global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) 
     U.at = U.end;
   }
 
-  // this lane's rows: column m32 of the wavefront's NQ row tiles
-  f16x8 q[NQ][KS];
-  float rf[NQ];
-  int lo[NQ], hi[NQ];
+  // this lane's row: column m32 of the wavefront's row tile
+  f16x8 q[KS];
+  int lo, hi;
+  const int rr = 32 * wave + m32, row = T.r0 + rr;
+  const bool real = row < T.rows;
+  const int token = real ? row / A.group : 0, gq = real ? row - token * A.group : 0;
+  kv_visible(A, T, token, real, lo, hi);
+  const float rf = many_q<IO, D>(A, T.s0 + token, h * A.group + gq, hh, real, q);
+  f32x16 o[DT];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = T.r0 + 32 * (NQ * wave + n) + m32;
-    const bool real = r < T.rows;
-    const int i = real ? r / A.group : 0, gq = real ? r - i * A.group : 0;
-    kv_visible(A, T, i, real, lo[n], hi[n]);
-    rf[n] = many_q<IO, D>(A, T.s0 + i, h * A.group + gq, hh, real, q[n]);
-  }
-  f32x16 o[NQ][DT];
-  float mx[NQ], l[NQ];
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    mx[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) o[n][d][k] = 0.f;
-  }
+    for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
+  // Weights are e^(s - ref) vs: ref is 2^12 below the largest exponent seen when it was set, and is
+  // set anew only where a weight would pass 2^KV_FAR, so that most tiles need no maximum over a row's lanes.
+  float ref = KV_NONE, l = 0.f;
 
-  // Staging: thread t holds, of each 256 chunks of 16 codes of a tile, K chunk t (key t / (D / 16)) and V
+  // Staging: thread t holds, of each THREADS chunks of 16 codes of a tile, K chunk t (key t / (D / 16)) and V
   // chunk t (value t / 4, keys 16 (t % 4) ..).  Lane e of a wavefront holds table entry ids0 + e.
   const int32_t* table = S.table + (int64_t)T.b * S.ld;
   int ids = -1, ids0 = INT32_MIN / 2;
@@ -114,18 +110,20 @@ __global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) 
       for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? page[e] : p;
       return ((int64_t)p * C.heads + h) * (bs * D);
     };
+    if (4 * D < THREADS && tid >= 4 * D) return;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int at = tid + 256 * c, key = at / KS, part = at % KS;
+      const int at = tid + THREADS * c, key = at / KS, part = at % KS;
       kw[c] = *reinterpret_cast<const u32x4*>(C.k + pick(key >> 4) + ((tile * 64 + key) & (bs - 1)) * D + 16 * part);
       const int d = at >> 2, group = at & 3;
       vw[c] = *reinterpret_cast<const u32x4*>(C.v + pick(group) + d * bs + ((tile * 64 + 16 * group) & (bs - 1)));
     }
   };
   auto store = [&](int tile, int buf) {
+    if (4 * D < THREADS && tid >= 4 * D) return;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int at = tid + 256 * c, key = at / KS, part = at % KS, d = at >> 2, group = at & 3;
+      const int at = tid + THREADS * c, key = at / KS, part = at % KS, d = at >> 2, group = at & 3;
       f16x8 x, y;
       to_halves<CODES>(kw[c], x, y);
       *reinterpret_cast<f16x8*>(&lds[buf][swizzled<2 * D>(key, 2 * part)]) = x;
@@ -159,120 +157,116 @@ __global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) 
     for (int e = 0; e < NP; ++e) { ks[e] = ks_n[e]; vs[e] = vs_n[e]; }
     load(min(tile + 1, z - 1));
     const int t0 = tile * 64;
-    bool any = false;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) any |= (t0 < hi[n]) & (t0 + 64 > lo[n]);
-    if (__any(any)) {
-      f32x16 s[NQ][2];
+    if (__any((t0 < hi) & (t0 + 64 > lo))) {
+      const uint8_t* const kb = lds[buf];
+      const uint8_t* const vb = lds[buf] + KB;
+      f32x16 s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        f16x8 ka[KS];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int c = 0; c < KS; ++c) ka[c] = *reinterpret_cast<const f16x8*>(kb + swizzled<2 * D>(32 * t + mk, 2 * c + hh));
 #pragma unroll
-          for (int k = 0; k < 16; ++k) s[n][t][k] = 0.f;
+        for (int k = 0; k < 16; ++k) s[t][k] = 0.f;
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          const f16x8 ka = *reinterpret_cast<const f16x8*>(&lds[buf][swizzled<2 * D>(32 * t + mk, 2 * c + hh)]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, q[n][c], s[n][t], 0, 0, 0);
-        }
+        for (int c = 0; c < KS; ++c) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], q[c], s[t], 0, 0, 0);
       }
-      float lv[4], iv[4], kq[4];
+      float lv[NP], iv[NP], kq[NP];
       bool vbad = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = vs[e * NP / 4];
-        const bool bad = mag(v) >= 0x7f800000u;
+      for (int e = 0; e < NP; ++e) {
+        const bool bad = mag(vs[e]) >= 0x7f800000u;
         vbad |= bad;
-        const float vq = bad ? 1.f : fmaxf(v, KV_SCALE_MIN);
+        const float vq = bad ? 1.f : fmaxf(vs[e], KV_SCALE_MIN);
         lv[e] = __builtin_amdgcn_logf(vq);
-        iv[e] = 1.0f / vq;
-        kq[e] = ks[e * NP / 4];
+        iv[e] = __builtin_amdgcn_rcpf(vq);
+        kq[e] = ks[e] * rf;
       }
-      f16x8 p[NQ][4];
+      const bool edge = __any((okv != 15) | (t0 < lo) | (t0 + 64 > hi));
+      float e[4][8], top = -INFINITY;
+      auto exponents = [&](float from) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float e[2][16], top = -INFINITY;
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int k = 0; k < 8; ++k) e[g][k] = s[g / 2][8 * (g & 1) + k] * kq[g * NP / 4] + (lv[g * NP / 4] - from);
+        if (edge) {
+          const int k0 = lo - t0 - 8 * hh, k1 = hi - t0 - 8 * hh;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) e[t][k] = s[n][t][k] * (kq[2 * t + k / 8] * rf[n]) + lv[2 * t + k / 8];
-        if (__any((okv != 15) | (t0 < lo[n]) | (t0 + 64 > hi[n]))) {
+          for (int g = 0; g < 4; ++g) {
+            const int a0 = okv >> g & 1 ? k0 : 64;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int key = t0 + 32 * t + 16 * (k / 8) + 8 * hh + k % 8;
-              const bool see = (okv >> (2 * t + k / 8) & 1) & (key >= lo[n]) & (key < hi[n]);
-              e[t][k] = see ? e[t][k] : -INFINITY;
-            }
+            for (int k = 0; k < 8; ++k) e[g][k] = ((16 * g + k >= a0) & (16 * g + k < k1)) ? e[g][k] : -INFINITY;
+          }
         }
+        top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) top = fmaxf(top, e[t][k]);
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, e[g][k]);
+      };
+      exponents(ref);
+      if (__any(top > KV_FAR)) {
+        exponents(0.f);
         top = max_halves(top);
-        if (__any(top > mx[n])) {
-          const float mn = fmaxf(mx[n], top);
-          const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[n] - mn);
-          mx[n] = mn;
-          l[n] *= f;
+        const float next = fmaxf(ref, top - KV_NEAR);
+        const float f = __builtin_amdgcn_exp2f(ref - next);
+        ref = next;
+        l *= f;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) o[n][d] *= f;
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+        exponents(ref);
+      }
+      f16x8 p[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          const f32x2 w = {__builtin_amdgcn_exp2f(e[g][k]), __builtin_amdgcn_exp2f(e[g][k + 1])};
+          sum += w[0];
+          sum += w[1];
+          const f16x2 w16 = __builtin_convertvector(w, f16x2);
+          p[g][k] = w16[0];
+          p[g][k + 1] = w16[1];
         }
-        const float ref = (mx[n] == -INFINITY ? 0.f : mx[n]) - KV_P_LOG2;
+        l += sum * iv[g * NP / 4];
+      }
+      if (vbad) {                                              // the same in every lane
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float sum = 0.f;
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float w = __builtin_amdgcn_exp2f(e[g / 2][8 * (g & 1) + k] - ref);
-            sum += w;
-            p[n][g][k] = (f16)w;
+            const int key = t0 + 16 * g + 8 * hh + k;
+            const bool see = (okv >> g & 1) & (key >= lo) & (key < hi) & (mag(vs[g * NP / 4]) >= 0x7f800000u);
+            p[g][k] = see ? (f16)NAN : p[g][k];
           }
-          l[n] += sum * iv[g];
-        }
-        if (__any(vbad)) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int key = t0 + 16 * g + 8 * hh + k;
-              const bool see = (okv >> g & 1) & (key >= lo[n]) & (key < hi[n]) & (mag(vs[g * NP / 4]) >= 0x7f800000u);
-              p[n][g][k] = see ? (f16)NAN : p[n][g][k];
-            }
-        }
       }
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < 4; ++g) {
+        f16x8 va[DT];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const f16x8 va = *reinterpret_cast<const f16x8*>(&lds[buf][KB + swizzled<128>(32 * d + m32, 2 * g + hh)]);
+        for (int d = 0; d < DT; ++d) va[d] = *reinterpret_cast<const f16x8*>(vb + swizzled<128>(32 * d + m32, 2 * g + hh));
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, p[n][g], o[n][d], 0, 0, 0);
-        }
+        for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[d], p[g], o[d], 0, 0, 0);
+      }
     }
     store(tile + 1, buf ^ 1);
     __syncthreads();
   }
 
-  // a lane holds values 32 d + 8 k + 4 hh + 0..3 of its rows
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_halves(l[n]);
-    const int rr = 32 * (NQ * wave + n) + m32, r = T.r0 + rr;
-    if (r >= T.rows) continue;
+  // a lane holds values 32 d + 8 k + 4 hh + 0..3 of its row
+  l = sum_halves(l);
+  if (real) {
     if (runs == 1) {
-      const int i = r / A.group;
-      const int64_t at = (int64_t)(T.s0 + i) * A.q_heads + h * A.group + (r - i * A.group);
-      const float inv = kv_inverse(l[n]);
+      const int64_t at = (int64_t)(T.s0 + token) * A.q_heads + h * A.group + gq;
+      const float inv = kv_inverse(l);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           store4<IO>(A.out + at * D + 32 * d + 8 * k + 4 * hh,
-                     f32x4{o[n][d][4 * k] * inv, o[n][d][4 * k + 1] * inv, o[n][d][4 * k + 2] * inv, o[n][d][4 * k + 3] * inv});
-      if (A.lse && hh == 0) A.lse[at] = kv_lse(mx[n], l[n]);
+                     f32x4{o[d][4 * k] * inv, o[d][4 * k + 1] * inv, o[d][4 * k + 2] * inv, o[d][4 * k + 3] * inv});
+      if (A.lse && hh == 0) A.lse[at] = kv_lse(ref + KV_P_LOG2, l);
     } else {
       // workgroup owner + i has part i; the owner's is its second
       float* part = A.parts + (((int64_t)h * A.shares + blockIdx.x) * 2 + (run == 0)) * R * (D + 4) + (int64_t)rr * (D + 4);
@@ -281,10 +275,10 @@ __global__ __launch_bounds__(256, 1) void kv_attn_many_kernel(const AttnArgs A) 
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           *reinterpret_cast<f32x4*>(part + 32 * d + 8 * k + 4 * hh) =
-              f32x4{o[n][d][4 * k], o[n][d][4 * k + 1], o[n][d][4 * k + 2], o[n][d][4 * k + 3]};
+              f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
       if (hh == 0) {
-        part[D] = mx[n];
-        part[D + 1] = l[n];
+        part[D] = ref + KV_P_LOG2;
+        part[D + 1] = l;
       }
     }
   }
@@ -325,17 +319,17 @@ __global__ __launch_bounds__(256) void kv_attn_many_join_kernel(const AttnArgs A
 template <int CODES, typename IO, int D>
 static int many_launch(const AttnArgs& A, const AttnPlan& P, hipStream_t st) {
   const dim3 grid((unsigned)P.grid, (unsigned)A.C.heads);
-  auto pick = [&](auto nq) {
-    constexpr int NQ = decltype(nq)::value;
-    auto kern = A.C.block >= 64 ? kv_attn_many_kernel<CODES, IO, D, NQ, 1>
-                : A.C.block == 32 ? kv_attn_many_kernel<CODES, IO, D, NQ, 2> : kv_attn_many_kernel<CODES, IO, D, NQ, 4>;
-    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, A);
+  auto pick = [&](auto waves) {
+    constexpr int WAVES = decltype(waves)::value;
+    auto kern = A.C.block >= 64 ? kv_attn_many_kernel<CODES, IO, D, WAVES, 1>
+                : A.C.block == 32 ? kv_attn_many_kernel<CODES, IO, D, WAVES, 2> : kv_attn_many_kernel<CODES, IO, D, WAVES, 4>;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), 0, st, A);
   };
   if constexpr (D <= 128) {
-    if (P.rows == 256) pick(std::integral_constant<int, 2>());
-    else pick(std::integral_constant<int, 1>());
+    if (P.rows == 256) pick(std::integral_constant<int, 8>());
+    else pick(std::integral_constant<int, 4>());
   } else {
-    pick(std::integral_constant<int, 1>());
+    pick(std::integral_constant<int, 4>());
   }
   PP_LAUNCH_CHECK();
   if (P.shares) {
