@@ -225,6 +225,18 @@ __device__ __forceinline__ float sum_groups(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return uniform(v);
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
+// A value that every lane wants and that no kernel of the launch writes, through the scalar cache.
+__device__ __forceinline__ float scalar_load(const float* p) {
+  return *(const __attribute__((address_space(4))) float*)uniform_ptr(p);
+}
+
 // Over the lanes l, l ^ 32.
 __device__ __forceinline__ float max_halves(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -8,25 +8,31 @@
 // which row of the product is free: row m takes the key whose bits 2 and 3 are those of m swapped, so
 // that the 8 scores of a lane that make one operand of O^T = V^T P^T belong to 8 consecutive keys,
 // 16 c + 8 (lane / 32) + 0..7, and V's operand is one 16-byte read of a row of the transposed V.
-// LDS rows are swizzled in 16-byte chunks so that 16 lanes of a read touch every bank once.
 #include "kv_attn.h"
 
 namespace pp {
 
-constexpr float KV_NONE = -1e30f, KV_NEAR = 12.f, KV_FAR = 15.9f;
-
-// 16-byte chunk c of row r: rows of a multiple of 256 bytes by r % 16, of an odd multiple of 128 by r / 2 % 8.
-template <int BYTES>
-__device__ __forceinline__ int swizzled(int r, int c) {
-  return BYTES % 256 == 0 ? r * BYTES + 16 * (c ^ (r & 15)) : r * BYTES + 16 * (c ^ ((r >> 1) & 7));
+// A barrier that nothing is scheduled across.
+__device__ __forceinline__ void phase() {
+  __builtin_amdgcn_sched_barrier(0);
+  __syncthreads();
+  __builtin_amdgcn_sched_barrier(0);
 }
+
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+constexpr float KV_NONE = -1e30f, KV_NEAR = 12.f, KV_FAR = 65000.f;
 
 template <int CODES, typename IO, int D, int WAVES, int NP>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(const AttnArgs A) {
   constexpr int KS = D / 16, DT = D / 32, R = 32 * WAVES, THREADS = 64 * WAVES;
   constexpr int CH = 4 * D < THREADS ? 1 : 4 * D / THREADS;            // chunks of 16 codes of K and of V a thread stages
-  constexpr int KB = 64 * D * 2;                                       // bytes of a tile of K or V
-  __shared__ __align__(16) uint8_t lds[2][2 * KB];
+  constexpr bool PING = WAVES == 8;
+  // Rows in LDS are 16 bytes longer than their halves, so that 16 rows' chunks of a column lie in all the banks
+  // and every chunk of an operand is one address and a constant.
+  constexpr int KR = 2 * D + 16, VR = 2 * 64 + 16, KB = 64 * KR, VB = D * VR, RING = PING ? 3 : 2;
+  __shared__ __align__(16) uint8_t lds[RING * (KB + VB)];
   const KvCache& C = A.C;
   const KvSeqs& S = A.S;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), m32 = lane & 31, hh = lane >> 5;
@@ -70,66 +76,82 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
   const int token = real ? row / A.group : 0, gq = real ? row - token * A.group : 0;
   kv_visible(A, T, token, real, lo, hi);
   const float rf = many_q<IO, D>(A, T.s0 + token, h * A.group + gq, hh, real, q);
+  if (!real) hi = T.lim;                                     // a row that is not there needs no mask
+  const int all_lo = wave_max(lo), all_hi = wave_min(hi);    // keys that all the wavefront's rows see
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
-  // Weights are e^(s - ref) vs: ref is 2^12 below the largest exponent seen when it was set, and is
-  // set anew only where a weight would pass 2^KV_FAR, so that most tiles need no maximum over a row's lanes.
+  // Weights are e^(s - ref) vs: ref was the largest exponent less 12 when it was set, and is set anew
+  // only where the weights of 8 keys pass what fp16 holds, so that most tiles need no maximum.
   float ref = KV_NONE, l = 0.f;
 
   // Staging: thread t holds, of each THREADS chunks of 16 codes of a tile, K chunk t (key t / (D / 16)) and V
   // chunk t (value t / 4, keys 16 (t % 4) ..).  Lane e of a wavefront holds table entry ids0 + e.
   const int32_t* table = S.table + (int64_t)T.b * S.ld;
   int ids = -1, ids0 = INT32_MIN / 2;
-  u32x4 kw[CH], vw[CH];
-  float ks_n[NP], vs_n[NP];
-  int ok_n = 0;
-  auto load = [&](int tile) {
-    const int e0 = (tile * 64) >> shift;
+  struct Pages {
+    int p[NP];
+  };
+  auto pages = [&](int tile) {                               // of the tile, or of the last one
+    const int e0 = (min(tile, z - 1) * 64) >> shift;
     if (e0 < ids0 || e0 + NP > ids0 + 64) {
       ids0 = e0;
       ids = (int64_t)e0 + lane < S.width ? table[e0 + lane] : -1;
       ids = ids < C.pages ? ids : -1;
     }
-    int page[NP];
-    ok_n = 0;
+    Pages P;
 #pragma unroll
-    for (int e = 0; e < NP; ++e) {
-      page[e] = lane_read(ids, e0 - ids0 + e);
-      ok_n |= (page[e] >= 0 ? (1 << (4 / NP)) - 1 : 0) << (4 / NP * e);
-      page[e] = page[e] < 0 ? 0 : page[e];
-      const int64_t ph = (int64_t)page[e] * C.heads + h;
-      ks_n[e] = C.ks[ph];
-      vs_n[e] = C.vs[ph];
-    }
-    auto pick = [&](int group) {
-      int p = page[0];
+    for (int e = 0; e < NP; ++e) P.p[e] = lane_read(ids, e0 - ids0 + e);
+    return P;
+  };
+  auto base = [&](const Pages& P, int group) {               // of the page that holds keys 16 group .. of the tile
+    int p = P.p[0];
 #pragma unroll
-      for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? page[e] : p;
-      return ((int64_t)p * C.heads + h) * (bs * D);
-    };
-    if (4 * D < THREADS && tid >= 4 * D) return;
+    for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? P.p[e] : p;
+    return ((int64_t)(p < 0 ? 0 : p) * C.heads + h) * (bs * D);
+  };
+  u32x4 kw[CH], vw[CH];
+  const bool stages = 4 * D >= THREADS || tid < 4 * D;
+  auto load_k = [&](const Pages& P, int tile) {
+    if (!stages) return;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = tid + THREADS * c, key = at / KS, part = at % KS;
-      kw[c] = *reinterpret_cast<const u32x4*>(C.k + pick(key >> 4) + ((tile * 64 + key) & (bs - 1)) * D + 16 * part);
-      const int d = at >> 2, group = at & 3;
-      vw[c] = *reinterpret_cast<const u32x4*>(C.v + pick(group) + d * bs + ((tile * 64 + 16 * group) & (bs - 1)));
+      kw[c] = *reinterpret_cast<const u32x4*>(C.k + base(P, key >> 4) + ((tile * 64 + key) & (bs - 1)) * D + 16 * part);
     }
   };
-  auto store = [&](int tile, int buf) {
-    if (4 * D < THREADS && tid >= 4 * D) return;
+  auto load_v = [&](const Pages& P, int tile) {
+    if (!stages) return;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int at = tid + THREADS * c, key = at / KS, part = at % KS, d = at >> 2, group = at & 3;
+      const int at = tid + THREADS * c, d = at >> 2, group = at & 3;
+      vw[c] = *reinterpret_cast<const u32x4*>(C.v + base(P, group) + d * bs + ((tile * 64 + 16 * group) & (bs - 1)));
+    }
+  };
+  auto store_k = [&](int at_ring) {
+    if (!stages) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = tid + THREADS * c, key = at / KS, part = at % KS;
       f16x8 x, y;
       to_halves<CODES>(kw[c], x, y);
-      *reinterpret_cast<f16x8*>(&lds[buf][swizzled<2 * D>(key, 2 * part)]) = x;
-      *reinterpret_cast<f16x8*>(&lds[buf][swizzled<2 * D>(key, 2 * part + 1)]) = y;
-      if (CODES == PP_KV_E4M3) {                 // codes past the length may be NaN
-        const int seen = ok_n >> group & 1 ? T.lim - tile * 64 - 16 * group : 0;
+      uint8_t* const k = lds + at_ring * KB + key * KR + 32 * part;
+      *reinterpret_cast<f16x8*>(k) = x;
+      *reinterpret_cast<f16x8*>(k + 16) = y;
+    }
+  };
+  auto store_v = [&](const Pages& P, int tile, int at_ring) {
+    if (!stages) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = tid + THREADS * c, d = at >> 2, group = at & 3;
+      if (CODES == PP_KV_E4M3) {                             // codes past the length may be NaN
+        int p = P.p[0];
+#pragma unroll
+        for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? P.p[e] : p;
+        const int seen = p >= 0 ? T.lim - tile * 64 - 16 * group : 0;
         if (seen < 16) {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -138,120 +160,201 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
           }
         }
       }
+      f16x8 x, y;
       to_halves<CODES>(vw[c], x, y);
-      *reinterpret_cast<f16x8*>(&lds[buf][KB + swizzled<128>(d, 2 * group)]) = x;
-      *reinterpret_cast<f16x8*>(&lds[buf][KB + swizzled<128>(d, 2 * group + 1)]) = y;
+      uint8_t* const v = lds + RING * KB + at_ring * VB + d * VR + 32 * group;
+      *reinterpret_cast<f16x8*>(v) = x;
+      *reinterpret_cast<f16x8*>(v + 16) = y;
     }
+  };
+  struct Scales {
+    float k[NP], v[NP];
+    int ok;
+  };
+  auto scales = [&](const Pages& P) {
+    Scales X;
+    X.ok = 0;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      const int64_t ph = (int64_t)(P.p[e] < 0 ? 0 : P.p[e]) * C.heads + h;
+      X.k[e] = scalar_load(C.ks + ph);
+      X.v[e] = scalar_load(C.vs + ph);
+      X.ok |= (P.p[e] >= 0 ? (1 << (4 / NP)) - 1 : 0) << (4 / NP * e);
+    }
+    return X;
   };
 
   const int mk = (m32 & 0x13) | (m32 & 4) << 1 | (m32 & 8) >> 1;       // key of row m32: bits 2 and 3 swapped
+  const uint8_t* const kl = lds + mk * KR + 16 * hh;
+  const uint8_t* const vl = lds + RING * KB + m32 * VR + 16 * hh;
+  f32x16 s[2];
+  f16x8 p[4];
+
+  // One step of a wavefront: the weights of tile i and the staging of later tiles, a barrier, the products
+  // (the weighted values of tile i and the scores of tile i + 1), a barrier.  With 8 wavefronts
+  // the second four, which share the SIMDs with the first, run one barrier behind, so that one
+  // wavefront of a SIMD has the matrix cores while the other has the vector unit.  Operands are read
+  // from LDS a group of products ahead, and no further: all at once they would not leave
+  // registers for the sums.
+  f16x8 va[2][DT], ka[2][4];
+  auto read_v = [&](auto buf, const uint8_t* v, int g) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) va[decltype(buf)::value][d] = *reinterpret_cast<const f16x8*>(v + 32 * d * VR + 32 * g);
+  };
+  auto read_k = [&](auto buf, const uint8_t* k, int c) {      // chunks c and c + 1
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      ka[decltype(buf)::value][e] = *reinterpret_cast<const f16x8*>(k + 32 * (e & 1) * KR + 32 * (c + (e >> 1)));
+  };
+  auto score = [&](auto buf, int c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      s[e & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[decltype(buf)::value][e], q[c + (e >> 1)],
+                                                        c + (e >> 1) == 0 ? f32x16{} : s[e & 1], 0, 0, 0);
+  };
+  auto scores = [&](const uint8_t* k) {                       // the first group is read
+#pragma unroll
+    for (int c = 0; c < KS; c += 4) {
+      read_k(Int<1>(), k, c + 2);
+      score(Int<0>(), c);
+      __builtin_amdgcn_sched_barrier(0);
+      if (c + 4 < KS) read_k(Int<0>(), k, c + 4);
+      score(Int<1>(), c + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto value = [&](auto buf, int g) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[decltype(buf)::value][d], p[g], o[d], 0, 0, 0);
+  };
+  auto products = [&](const uint8_t* v, const uint8_t* k) {
+    read_v(Int<0>(), v, 0);
+    read_v(Int<1>(), v, 1);
+    value(Int<0>(), 0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(Int<0>(), v, 2);
+    value(Int<1>(), 1);
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(Int<1>(), v, 3);
+    value(Int<0>(), 2);
+    __builtin_amdgcn_sched_barrier(0);
+    read_k(Int<0>(), k, 0);
+    value(Int<1>(), 3);
+    __builtin_amdgcn_sched_barrier(0);
+    scores(k);
+  };
+
   if (a < z) {
-    load(a);
-    store(a, 0);
-  }
-  __syncthreads();
-  for (int tile = a; tile < z; ++tile) {
-    const int buf = (tile - a) & 1, okv = ok_n;
-    float ks[NP], vs[NP];
-#pragma unroll
-    for (int e = 0; e < NP; ++e) { ks[e] = ks_n[e]; vs[e] = vs_n[e]; }
-    load(min(tile + 1, z - 1));
-    const int t0 = tile * 64;
-    if (__any((t0 < hi) & (t0 + 64 > lo))) {
-      const uint8_t* const kb = lds[buf];
-      const uint8_t* const vb = lds[buf] + KB;
-      f32x16 s[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f16x8 ka[KS];
-#pragma unroll
-        for (int c = 0; c < KS; ++c) ka[c] = *reinterpret_cast<const f16x8*>(kb + swizzled<2 * D>(32 * t + mk, 2 * c + hh));
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s[t][k] = 0.f;
-#pragma unroll
-        for (int c = 0; c < KS; ++c) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], q[c], s[t], 0, 0, 0);
-      }
+    Pages p1 = pages(a), p2 = pages(a + 1), p3;
+    load_k(p1, a);
+    load_v(p1, a);
+    Scales sc = scales(p1);
+    store_k(0);
+    store_v(p1, a, 0);
+    load_k(p2, min(a + 1, z - 1));
+    store_k(1);
+    p3 = pages(a + 2);
+    load_k(p3, min(a + 2, z - 1));
+    load_v(p2, min(a + 1, z - 1));
+    __syncthreads();
+    read_k(Int<0>(), kl, 0);
+    scores(kl);
+    if (PING && wave >= WAVES / 2) phase();
+    int r0 = 0;                                               // ring of V of tile i, and of K
+    for (int i = a; i < z; ++i) {
+      const int t0 = i * 64, r1 = r0 + 1 == RING ? 0 : r0 + 1, r2 = r1 + 1 == RING ? 0 : r1 + 1;
+      const Scales sn = scales(p2);
       float lv[NP], iv[NP], kq[NP];
       bool vbad = false;
+      const float from = ref == KV_NONE ? 0.f : ref;
 #pragma unroll
       for (int e = 0; e < NP; ++e) {
-        const bool bad = mag(vs[e]) >= 0x7f800000u;
+        const bool bad = mag(sc.v[e]) >= 0x7f800000u;
         vbad |= bad;
-        const float vq = bad ? 1.f : fmaxf(vs[e], KV_SCALE_MIN);
-        lv[e] = __builtin_amdgcn_logf(vq);
+        const float vq = bad ? 1.f : fmaxf(sc.v[e], KV_SCALE_MIN);
+        lv[e] = __builtin_amdgcn_logf(vq) - from;
         iv[e] = __builtin_amdgcn_rcpf(vq);
-        kq[e] = ks[e] * rf;
+        kq[e] = sc.k[e] * rf;
       }
-      const bool edge = __any((okv != 15) | (t0 < lo) | (t0 + 64 > hi));
-      float e[4][8], top = -INFINITY;
-      auto exponents = [&](float from) {
+      float sum[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) e[g][k] = s[g / 2][8 * (g & 1) + k] * kq[g * NP / 4] + (lv[g * NP / 4] - from);
-        if (edge) {
-          const int k0 = lo - t0 - 8 * hh, k1 = hi - t0 - 8 * hh;
+        for (int k = 0; k < 8; ++k)
+          s[g / 2][8 * (g & 1) + k] = s[g / 2][8 * (g & 1) + k] * kq[g * NP / 4] + lv[g * NP / 4];
+      const int k0 = lo - t0 - 8 * hh, k1 = hi - t0 - 8 * hh;   // the row's keys, 16 g + k of them this lane's
+      if ((sc.ok != 15) | (t0 < all_lo) | (t0 + 64 > all_hi)) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int a0 = okv >> g & 1 ? k0 : 64;
+        for (int g = 0; g < 4; ++g) {
+          const int a0 = sc.ok >> g & 1 ? k0 : 64;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[g][k] = ((16 * g + k >= a0) & (16 * g + k < k1)) ? e[g][k] : -INFINITY;
+          for (int k = 0; k < 8; ++k) {
+            const int at = 8 * (g & 1) + k;
+            s[g / 2][at] = ((16 * g + k >= a0) & (16 * g + k < k1)) ? s[g / 2][at] : -INFINITY;
           }
         }
-        top = -INFINITY;
+      }
+      auto weights = [&]() {
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 4; ++g) {
+          sum[g] = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) top = fmaxf(top, e[g][k]);
+          for (int k = 0; k < 8; k += 2) {
+            const int at = 8 * (g & 1) + k;
+            const f32x2 w = {__builtin_amdgcn_exp2f(s[g / 2][at]), __builtin_amdgcn_exp2f(s[g / 2][at + 1])};
+            sum[g] += w[0];
+            sum[g] += w[1];
+            const f16x2 w16 = __builtin_convertvector(w, f16x2);
+            p[g][k] = w16[0];
+            p[g][k + 1] = w16[1];
+          }
+        }
       };
-      exponents(ref);
-      if (__any(top > KV_FAR)) {
-        exponents(0.f);
-        top = max_halves(top);
-        const float next = fmaxf(ref, top - KV_NEAR);
+      weights();
+      const float most = fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3]));
+      if (__any((ref == KV_NONE) | (most > KV_FAR))) {       // for the rows that need it: no row sways another
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+        const bool need = (ref == KV_NONE) | (max_halves(most) > KV_FAR);
+        const float next = need ? fmaxf(ref, max_halves(top) + from - KV_NEAR) : ref;
         const float f = __builtin_amdgcn_exp2f(ref - next);
-        ref = next;
         l *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
-        exponents(ref);
-      }
-      f16x8 p[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          const f32x2 w = {__builtin_amdgcn_exp2f(e[g][k]), __builtin_amdgcn_exp2f(e[g][k + 1])};
-          sum += w[0];
-          sum += w[1];
-          const f16x2 w16 = __builtin_convertvector(w, f16x2);
-          p[g][k] = w16[0];
-          p[g][k + 1] = w16[1];
+        for (int e = 0; e < 16; ++e) {
+          s[0][e] += from - next;
+          s[1][e] += from - next;
         }
-        l += sum * iv[g * NP / 4];
+        ref = next;
+        weights();
       }
-      if (vbad) {                                              // the same in every lane
+#pragma unroll
+      for (int g = 0; g < 4; ++g) l += sum[g] * iv[g * NP / 4];
+      if (vbad) {                                            // the same in every lane
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const int key = t0 + 16 * g + 8 * hh + k;
-            const bool see = (okv >> g & 1) & (key >= lo) & (key < hi) & (mag(vs[g * NP / 4]) >= 0x7f800000u);
+            const bool see = (sc.ok >> g & 1) & (16 * g + k >= k0) & (16 * g + k < k1) &
+                             (mag(sc.v[g * NP / 4]) >= 0x7f800000u);
             p[g][k] = see ? (f16)NAN : p[g][k];
           }
       }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f16x8 va[DT];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) va[d] = *reinterpret_cast<const f16x8*>(vb + swizzled<128>(32 * d + m32, 2 * g + hh));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[d], p[g], o[d], 0, 0, 0);
-      }
+      store_v(p2, i + 1, r1);
+      store_k(r2);
+      p2 = p3;
+      p3 = pages(i + 3);
+      load_v(p2, min(i + 2, z - 1));
+      load_k(p3, min(i + 3, z - 1));
+      sc = sn;
+      phase();
+      products(vl + r0 * VB, kl + r1 * KB);
+      phase();
+      r0 = r1;
     }
-    store(tile + 1, buf ^ 1);
-    __syncthreads();
+    if (PING && wave < WAVES / 2) phase();
   }
 
   // a lane holds values 32 d + 8 k + 4 hh + 0..3 of its row
@@ -284,6 +387,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
   }
   if (runs > 1 && run == 0 && tid == 0) *desc = ManyPart{runs, T.s0, T.r0, min(R, T.rows - T.r0)};
   if (U.at >= U.end) return;
+  __syncthreads();                       // the rings are read
   }
 }
 
