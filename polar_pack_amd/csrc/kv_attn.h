@@ -72,6 +72,13 @@ __device__ __forceinline__ bool kv_tile_fill(const AttnArgs& A, int R, RowTile& 
   return true;
 }
 
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return uniform(v);
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
 // Work item `at` of the call: tiles of R rows, sequence after sequence.
 __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, RowTile& T) {
   if (A.S.cu == nullptr) {
@@ -84,6 +91,42 @@ __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, Ro
     T.r0 = (at - kv_begin(A.S, T.b, A.group, R, 1)) * R;
   }
   T.b = uniform(T.b);
+  return kv_tile_fill(A, R, T);
+}
+
+// Work item `at` with the row tiles that see the most keys first, so that the last workgroups to start are
+// short ones: every sequence's last row tile, then every one's last but one.  More sequences
+// than a wavefront has lanes come one after another.
+__device__ __forceinline__ bool kv_row_tile_from_last(const AttnArgs& A, int at, int R, RowTile& T) {
+  const KvSeqs& S = A.S;
+  if (S.batch > 63) {
+    const int items = (int)((int64_t)S.tokens * A.group / R) + S.batch + 1;
+    return kv_row_tile(A, items - 1 - at, R, T);
+  }
+  const int b = threadIdx.x & 63;
+  const int n = b <= S.batch ? kv_start(S, b + 1) - kv_start(S, b) : 0;
+  const int tiles = n > 0 ? (n * A.group + R - 1) / R : 0;
+  auto sum = [](int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return uniform(v);
+  };
+  int lo = 0, hi = wave_max(tiles);        // the round: the largest with sum of min(tiles, round) <= at
+  if (at >= sum(tiles)) return false;
+  int before = 0;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2, done = sum(min(tiles, mid));
+    if (done <= at) {
+      lo = mid;
+      before = done;
+    } else {
+      hi = mid;
+    }
+  }
+  uint64_t left = __ballot(tiles > lo);
+  for (int skip = at - before; skip > 0; --skip) left &= left - 1;
+  T.b = __builtin_ctzll(left);
+  T.r0 = (__builtin_amdgcn_readlane(tiles, T.b) - 1 - lo) * R;
   return kv_tile_fill(A, R, T);
 }
 
@@ -224,13 +267,6 @@ __device__ __forceinline__ float sum_groups(float v) {
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return uniform(v);
-}
-__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
 
 // A value that every lane wants and that no kernel of the launch writes, through the scalar cache.
 __device__ __forceinline__ float scalar_load(const float* p) {

@@ -22,6 +22,8 @@ __device__ __forceinline__ void phase() {
 template <int I>
 using Int = std::integral_constant<int, I>;
 
+typedef const __attribute__((address_space(1))) u32x4* GlobalCodes;    // not a flat address, whose loads wait for LDS
+
 constexpr float KV_NONE = -1e30f, KV_NEAR = 12.f, KV_FAR = 65000.f;
 
 template <int CODES, typename IO, int D, int WAVES, int NP>
@@ -36,7 +38,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
   const KvCache& C = A.C;
   const KvSeqs& S = A.S;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), m32 = lane & 31, hh = lane >> 5;
-  const int h = blockIdx.y, shift = C.shift, bs = C.block;
+  const int h = A.shares ? blockIdx.y : blockIdx.x % C.heads, shift = C.shift, bs = C.block;
   RowTile T;
   Deal U;
   ManyPart* const desc = A.desc ? A.desc + (int64_t)h * A.shares + blockIdx.x : nullptr;
@@ -44,8 +46,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
     if (tid == 0) desc->runs = 0;
     if (!kv_deal<THREADS>(A, R, T, U)) return;
   } else {
-    // the last row tiles first: they see the most keys
-    if (!kv_row_tile(A, gridDim.x - 1 - blockIdx.x, R, T)) return;
+    if (!kv_row_tile_from_last(A, blockIdx.x / C.heads, R, T)) return;
     U = Deal{0, 1, 1, T.lo >> 6, 1, 0};
   }
   for (;; kv_deal_next(A, R, T, U)) {
@@ -106,11 +107,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
     for (int e = 0; e < NP; ++e) P.p[e] = lane_read(ids, e0 - ids0 + e);
     return P;
   };
-  auto base = [&](const Pages& P, int group) {               // of the page that holds keys 16 group .. of the tile
+  // A page's codes of this head: its first tile's address the same in every lane where a tile lies in
+  // one page, so that a load is that and the thread's own offset.
+  auto codes = [&](const uint8_t* all, const Pages& P, int group, int in_page) {
     int p = P.p[0];
 #pragma unroll
     for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? P.p[e] : p;
-    return ((int64_t)(p < 0 ? 0 : p) * C.heads + h) * (bs * D);
+    const uint8_t* at = all + ((int64_t)(p < 0 ? 0 : p) * C.heads + h) * (bs * D) + in_page;
+    return NP == 1 ? uniform_ptr(at) : at;
   };
   u32x4 kw[CH], vw[CH];
   const bool stages = 4 * D >= THREADS || tid < 4 * D;
@@ -119,7 +123,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = tid + THREADS * c, key = at / KS, part = at % KS;
-      kw[c] = *reinterpret_cast<const u32x4*>(C.k + base(P, key >> 4) + ((tile * 64 + key) & (bs - 1)) * D + 16 * part);
+      const uint32_t mine = (key & (NP == 1 ? 63 : bs - 1)) * D + 16 * part;
+      kw[c] = *(GlobalCodes)(codes(C.k, P, key >> 4, NP == 1 ? ((tile * 64) & (bs - 1)) * D : 0) + mine);
     }
   };
   auto load_v = [&](const Pages& P, int tile) {
@@ -127,7 +132,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = tid + THREADS * c, d = at >> 2, group = at & 3;
-      vw[c] = *reinterpret_cast<const u32x4*>(C.v + base(P, group) + d * bs + ((tile * 64 + 16 * group) & (bs - 1)));
+      const uint32_t mine = d * bs + ((16 * group) & (NP == 1 ? 63 : bs - 1));
+      vw[c] = *(GlobalCodes)(codes(C.v, P, group, NP == 1 ? (tile * 64) & (bs - 1) : 0) + mine);
     }
   };
   auto store_k = [&](int at_ring) {
@@ -142,24 +148,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
       *reinterpret_cast<f16x8*>(k + 16) = y;
     }
   };
-  auto store_v = [&](const Pages& P, int tile, int at_ring) {
+  // Codes of e4m3 past the length, or of no page, may be NaN: zeros instead.
+  auto clear_v = [&](const Pages& P, int tile) {
+    if (CODES != PP_KV_E4M3) return;
+    bool all = (tile + 1) * 64 <= T.lim;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) all &= P.p[e] >= 0;
+    if (all) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int group = (tid + THREADS * c) & 3;
+      int p = P.p[0];
+#pragma unroll
+      for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? P.p[e] : p;
+      const int seen = p >= 0 ? T.lim - tile * 64 - 16 * group : 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int left = seen - 4 * w;
+        vw[c][w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+      }
+    }
+  };
+  auto store_v = [&](int at_ring) {
     if (!stages) return;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = tid + THREADS * c, d = at >> 2, group = at & 3;
-      if (CODES == PP_KV_E4M3) {                             // codes past the length may be NaN
-        int p = P.p[0];
-#pragma unroll
-        for (int e = 1; e < NP; ++e) p = group * NP / 4 == e ? P.p[e] : p;
-        const int seen = p >= 0 ? T.lim - tile * 64 - 16 * group : 0;
-        if (seen < 16) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int left = seen - 4 * w;
-            vw[c][w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-          }
-        }
-      }
       f16x8 x, y;
       to_halves<CODES>(vw[c], x, y);
       uint8_t* const v = lds + RING * KB + at_ring * VB + d * VR + 32 * group;
@@ -190,10 +204,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
   f32x16 s[2];
   f16x8 p[4];
 
-  // One step of a wavefront: the weights of tile i and the staging of later tiles, a barrier, the products
-  // (the weighted values of tile i and the scores of tile i + 1), a barrier.  With 8 wavefronts
+  // One step of a wavefront: the weights of tile i, a barrier, the products (the weighted values of
+  // tile i and the scores of tile i + 1) and beside them the staging of later tiles, a barrier.  With 8 wavefronts
   // the second four, which share the SIMDs with the first, run one barrier behind, so that one
-  // wavefront of a SIMD has the matrix cores while the other has the vector unit.  Operands are read
+  // wavefront of a SIMD has the matrix cores, and the priority, while the other has the vector unit.  Operands are read
   // from LDS a group of products ahead, and no further: all at once they would not leave
   // registers for the sums.
   f16x8 va[2][DT], ka[2][4];
@@ -227,30 +241,30 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[decltype(buf)::value][d], p[g], o[d], 0, 0, 0);
   };
-  auto products = [&](const uint8_t* v, const uint8_t* k) {
-    read_v(Int<0>(), v, 0);
-    read_v(Int<1>(), v, 1);
-    value(Int<0>(), 0);
-    __builtin_amdgcn_sched_barrier(0);
-    read_v(Int<0>(), v, 2);
-    value(Int<1>(), 1);
-    __builtin_amdgcn_sched_barrier(0);
-    read_v(Int<1>(), v, 3);
-    value(Int<0>(), 2);
-    __builtin_amdgcn_sched_barrier(0);
-    read_k(Int<0>(), k, 0);
-    value(Int<1>(), 3);
-    __builtin_amdgcn_sched_barrier(0);
-    scores(k);
+  // What a tile's scales make of its scores and sums, with the reference as it is.
+  float lv[NP], iv[NP], kq[NP], from = 0.f;
+  bool vbad = false;
+  auto weigh = [&](const Scales& X) {
+    from = ref == KV_NONE ? 0.f : ref;
+    vbad = false;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      const bool bad = mag(X.v[e]) >= 0x7f800000u;
+      vbad |= bad;
+      const float vq = bad ? 1.f : fmaxf(X.v[e], KV_SCALE_MIN);
+      lv[e] = __builtin_amdgcn_logf(vq) - from;
+      iv[e] = __builtin_amdgcn_rcpf(vq);
+      kq[e] = X.k[e] * rf;
+    }
   };
-
   if (a < z) {
     Pages p1 = pages(a), p2 = pages(a + 1), p3;
     load_k(p1, a);
     load_v(p1, a);
     Scales sc = scales(p1);
     store_k(0);
-    store_v(p1, a, 0);
+    clear_v(p1, a);
+    store_v(0);
     load_k(p2, min(a + 1, z - 1));
     store_k(1);
     p3 = pages(a + 2);
@@ -259,23 +273,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
     __syncthreads();
     read_k(Int<0>(), kl, 0);
     scores(kl);
+    weigh(sc);
     if (PING && wave >= WAVES / 2) phase();
     int r0 = 0;                                               // ring of V of tile i, and of K
     for (int i = a; i < z; ++i) {
       const int t0 = i * 64, r1 = r0 + 1 == RING ? 0 : r0 + 1, r2 = r1 + 1 == RING ? 0 : r1 + 1;
-      const Scales sn = scales(p2);
-      float lv[NP], iv[NP], kq[NP];
-      bool vbad = false;
-      const float from = ref == KV_NONE ? 0.f : ref;
-#pragma unroll
-      for (int e = 0; e < NP; ++e) {
-        const bool bad = mag(sc.v[e]) >= 0x7f800000u;
-        vbad |= bad;
-        const float vq = bad ? 1.f : fmaxf(sc.v[e], KV_SCALE_MIN);
-        lv[e] = __builtin_amdgcn_logf(vq) - from;
-        iv[e] = __builtin_amdgcn_rcpf(vq);
-        kq[e] = sc.k[e] * rf;
-      }
       float sum[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -342,15 +344,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
             p[g][k] = see ? (f16)NAN : p[g][k];
           }
       }
-      store_v(p2, i + 1, r1);
-      store_k(r2);
-      p2 = p3;
-      p3 = pages(i + 3);
-      load_v(p2, min(i + 2, z - 1));
-      load_k(p3, min(i + 3, z - 1));
-      sc = sn;
+      const Pages p4 = pages(i + 3);
+      clear_v(p2, i + 1);
       phase();
-      products(vl + r0 * VB, kl + r1 * KB);
+      __builtin_amdgcn_s_setprio(1);
+      const uint8_t* const v = vl + r0 * VB;
+      read_v(Int<0>(), v, 0);
+      read_v(Int<1>(), v, 1);
+      value(Int<0>(), 0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_v(Int<0>(), v, 2);
+      value(Int<1>(), 1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_v(Int<1>(), v, 3);
+      value(Int<0>(), 2);
+      load_v(p3, min(i + 2, z - 1));
+      __builtin_amdgcn_sched_barrier(0);
+      read_k(Int<0>(), kl + r1 * KB, 0);
+      value(Int<1>(), 3);
+      load_k(p4, min(i + 3, z - 1));
+      sc = scales(p2);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(kl + r1 * KB);
+      weigh(sc);
+      p2 = p3;
+      p3 = p4;
+      __builtin_amdgcn_s_setprio(0);
       phase();
       r0 = r1;
     }
@@ -422,7 +441,7 @@ __global__ __launch_bounds__(256) void kv_attn_many_join_kernel(const AttnArgs A
 
 template <int CODES, typename IO, int D>
 static int many_launch(const AttnArgs& A, const AttnPlan& P, hipStream_t st) {
-  const dim3 grid((unsigned)P.grid, (unsigned)A.C.heads);
+  const dim3 grid((unsigned)(P.shares ? P.grid : P.grid * A.C.heads), P.shares ? (unsigned)A.C.heads : 1u);
   auto pick = [&](auto waves) {
     constexpr int WAVES = decltype(waves)::value;
     auto kern = A.C.block >= 64 ? kv_attn_many_kernel<CODES, IO, D, WAVES, 1>
