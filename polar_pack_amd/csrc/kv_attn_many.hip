@@ -346,6 +346,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
       }
       const Pages p4 = pages(i + 3);
       clear_v(p2, i + 1);
+      store_v(r1);
+      store_k(r2);
       phase();
       __builtin_amdgcn_s_setprio(1);
       const uint8_t* const v = vl + r0 * VB;
