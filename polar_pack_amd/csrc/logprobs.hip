@@ -73,8 +73,25 @@ struct LpLds<false> { typedef LpNone type; };
 __device__ __forceinline__ const uint64_t* lp_best(const LpShared& L) { return L.best; }
 __device__ __forceinline__ const uint64_t* lp_best(const LpNone&) { return nullptr; }
 
-// Keys of `list` at or above a bound that k of them reach move to its front: the k-th largest of 64
-// groups' maxima (key i in group i % 64).  Twice the same threads, so that no key is lost between.
+// Raises the floor to the k-th largest of 64 groups' largest keys (thread t's in group t % 64): k keys at
+// least reach it.
+__device__ __forceinline__ void lp_floor(LpShared& L, uint64_t top, int k) {
+  const int tid = threadIdx.x;
+  if (tid < 64) L.group[tid] = 0;
+  __syncthreads();
+  atomicMax((unsigned long long*)&L.group[tid & 63], (unsigned long long)top);
+  __syncthreads();
+  if (tid < 64) {
+    const uint64_t g = L.group[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) rank += L.group[i] > g || (L.group[i] == g && i < tid);
+    if (rank == k - 1 && g > L.floor) L.floor = g;
+  }
+  __syncthreads();
+}
+
+// Keys of `list` below a floor that k of them reach leave it.
 __device__ __forceinline__ void lp_tidy(LpShared& L, int k) {
   const int tid = threadIdx.x;
   const int n = L.count;
@@ -87,18 +104,8 @@ __device__ __forceinline__ void lp_tidy(LpShared& L, int k) {
     top = mine[i] > top ? mine[i] : top;
   }
   __syncthreads();
-  if (tid < 64) L.group[tid] = 0;
   if (tid == 0) L.count = 0;
-  __syncthreads();
-  atomicMax((unsigned long long*)&L.group[tid & 63], (unsigned long long)top);
-  __syncthreads();
-  if (tid < 64) {
-    const uint64_t g = L.group[tid];
-    int rank = 0;
-    for (int i = 0; i < 64; ++i) rank += L.group[i] > g || (L.group[i] == g && i < tid);
-    if (rank == k - 1) L.floor = g > L.floor ? g : L.floor;
-  }
-  __syncthreads();
+  lp_floor(L, top, k);
   const uint64_t fl = L.floor;
 #pragma unroll
   for (int i = 0; i < (LP_LIST + LP_THREADS - 1) / LP_THREADS; ++i)
@@ -184,24 +191,30 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs A) {
     if (tid == 0) { L.count = 0; L.floor = 0; }
     __syncthreads();
   }
-  for (int c = lo; c < hi; c += LP_STEP) {
+  // The logits of the next two steps are on their way while a step's are worked on.
+  constexpr int LOADS = LP_PER / VE;
+  auto fetch = [&](u32x4* w, int c) {
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int at = c + (u * LP_THREADS + tid) * VE - skew;   // first logit of the load
+      if (at >= 0 && at + VE <= A.V && c < hi) {
+        w[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + at));
+      } else {
+        raw e[VE];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) e[i] = c < hi && at + i >= 0 && at + i < A.V ? x[at + i] : IO::put(-INFINITY);
+        __builtin_memcpy(&w[u], e, 16);
+      }
+    }
+  };
+  auto step = [&](const u32x4* w, int c) {
     float f[LP_PER];
 #pragma unroll
-    for (int u = 0; u < LP_PER / VE; ++u) {
-      const int at = c + (u * LP_THREADS + tid) * VE - skew;   // first logit of the load
-      if (at >= 0 && at + VE <= A.V) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(x + at);
-        if (sizeof(raw) == 4) {
+    for (int u = 0; u < LOADS; ++u) {
+      raw e[VE];
+      __builtin_memcpy(e, &w[u], 16);
 #pragma unroll
-          for (int i = 0; i < VE; ++i) f[u * VE + i] = __uint_as_float(w[i % 4]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) f[u * VE + i] = IO::get((raw)(w[(i / 2) % 4] >> (16 * (i & 1))));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) f[u * VE + i] = at + i >= 0 && at + i < A.V ? IO::get(x[at + i]) : -INFINITY;
-      }
+      for (int i = 0; i < VE; ++i) f[u * VE + i] = IO::get(e[i]);
     }
     float top = f[0];
 #pragma unroll
@@ -222,20 +235,47 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs A) {
       v.t += lp_far(d) * e;
     }
     if constexpr (TOP) {
+      auto each = [&](auto f2) {
+#pragma unroll
+        for (int u = 0; u < LP_PER / VE; ++u)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const int at = c + (u * LP_THREADS + tid) * VE - skew + i;
+            if (at >= 0 && at < A.V) f2(f[u * VE + i], at);
+          }
+      };
+      if (c == lo) {                                 // a first floor, so that the list starts short
+        uint64_t best = 0;
+        each([&](float x, int at) {
+          const uint64_t key = lp_key(x, at);
+          best = key > best ? key : best;
+        });
+        lp_floor(L, best, A.k);
+      }
       const uint64_t fl = L.floor;
-#pragma unroll
-      for (int u = 0; u < LP_PER / VE; ++u)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const int at = c + (u * LP_THREADS + tid) * VE - skew + i;
-          const uint64_t key = lp_key(f[u * VE + i], at);
-          if (at >= 0 && at < A.V && key >= fl) L.list[atomicAdd(&L.count, 1)] = key;
-        }
+      // few threads hold a candidate: a logit not below the floor's, or a NaN, which the sums show
+      const float least = lp_value(fl);              // a NaN while there is no floor: nothing is below it
+      if (!(top < least) || v.s != v.s)
+        each([&](float x, int at) {
+          if (x < least) return;
+          const uint64_t key = lp_key(x, at);
+          if (key >= fl) L.list[atomicAdd(&L.count, 1)] = key;
+        });
       __syncthreads();
       const int n = L.count;
       __syncthreads();                               // all have read the count before the next step adds to it
       if (n > LP_TIDY) lp_shorten(L, A.k);
     }
+  };
+  u32x4 w0[LOADS], w1[LOADS];
+  fetch(w0, lo);
+  fetch(w1, lo + LP_STEP);
+  for (int c = lo; c < hi; c += 2 * LP_STEP) {
+    step(w0, c);
+    fetch(w0, c + 2 * LP_STEP);
+    if (c + LP_STEP >= hi) break;
+    step(w1, c + LP_STEP);
+    fetch(w1, c + 3 * LP_STEP);
   }
   v = lp_block_join(v, sh);
   if constexpr (TOP) {
