@@ -16,7 +16,7 @@ namespace pp {
 constexpr int LP_THREADS = 256;
 constexpr int LP_PER = 16;                        // logits a thread and step
 constexpr int LP_STEP = LP_THREADS * LP_PER;
-constexpr int LP_TIDY = 256;                      // a longer list is picked after the step
+constexpr int LP_TIDY = 128;                      // a longer list is picked after the step
 constexpr int LP_LIST = LP_STEP + LP_TIDY;
 constexpr int LP_TOP_MAX = 64;
 
@@ -241,13 +241,13 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs A) {
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
             const int at = c + (u * LP_THREADS + tid) * VE - skew + i;
-            if (at >= 0 && at < A.V) f2(f[u * VE + i], at);
+            f2(f[u * VE + i], at);
           }
       };
       if (c == lo) {                                 // a first floor, so that the list starts short
         uint64_t best = 0;
         each([&](float x, int at) {
-          const uint64_t key = lp_key(x, at);
+          const uint64_t key = at >= 0 && at < A.V ? lp_key(x, at) : 0;
           best = key > best ? key : best;
         });
         lp_floor(L, best, A.k);
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(const LpArgs A) {
       const float least = lp_value(fl);              // a NaN while there is no floor: nothing is below it
       if (!(top < least) || v.s != v.s)
         each([&](float x, int at) {
-          if (x < least) return;
+          if (x < least || at < 0 || at >= A.V) return;
           const uint64_t key = lp_key(x, at);
           if (key >= fl) L.list[atomicAdd(&L.count, 1)] = key;
         });
