@@ -195,6 +195,24 @@ def test_many_sequences():
     check(1, 4, 64, 16, INT8, F16, lens, news)
 
 
+def test_more_sequences_than_are_dealt():
+    """Past 1,020 sequences every row tile is one workgroup's."""
+    g = torch.Generator().manual_seed(12)
+    lens = torch.randint(0, 90, (1100,), generator=g).tolist()
+    check(1, 4, 64, 64, INT8, F16, lens, [1] * 1100, cu=False)
+    check(1, 4, 64, 64, E4M3, F16, lens, [min(n, 2) for n in lens])
+
+
+@pytest.mark.parametrize("B,n", [(70, 68), (20, 240)])
+def test_many_row_tiles(B, n):
+    """Row tiles enough for every CU are not shared; those that see the most keys come first."""
+    g = torch.Generator().manual_seed(B)
+    news = torch.randint(n - 20, n + 20, (B,), generator=g).tolist()
+    news[3], news[5] = 1, 0
+    assert sum(news) * 32 / 256 >= 2 * torch.cuda.get_device_properties(DEV).multi_processor_count
+    check(1, 32, 64, 64, INT8, BF16, [m + 30 * (i % 3) for i, m in enumerate(news)], news, extra=3)
+
+
 def test_one_answer():
     """Joins do not depend on the order in which parts of a row end."""
     g = torch.Generator().manual_seed(3)
