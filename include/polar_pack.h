@@ -772,7 +772,8 @@ typedef struct pp_kv_cache {
  *   scale = max(old scale, max|x| / qmax, 2^-64),  qmax 127 or 448; the old scale counts if the
  *           page holds earlier tokens of the sequence, whose codes become round(code * (old / scale))
  *           where the scale grows;
- *   code  = round(x * (1 / scale)) held to +-qmax, in float32, ties to even.
+ *   code  = round(x * f) held to +-qmax, in float32, ties to even; f is qmax / max|x| where that sets
+ *           the scale, and 1 / scale otherwise.
  * A value that is not finite makes the page's scale not finite (and its codes 0), so that every row
  * that sees the page is NaN, until the page begins anew.  A page that gets tokens belongs to one
  * sequence of the call.

@@ -116,12 +116,15 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
   __syncthreads();
   for (int w = 0; w < (nthr + 63) / 64; ++w) top = max(top, red[w]);
   // unsigned order: scales are not negative, and a NaN stays
-  uint32_t bits = max(mag(__uint_as_float(top) / Q::kMax), max(mag(was), mag(KV_SCALE_MIN)));
+  const uint32_t need = mag(__uint_as_float(top) / Q::kMax);
+  const uint32_t bits = max(need, max(mag(was), mag(KV_SCALE_MIN)));
   const float now = __uint_as_float(bits);
   const bool finite = bits < 0x7f800000u;
   const bool grown = held && mag(was) < bits;
   const float ratio = finite ? was / now : 0.f;
-  const float inv = finite ? 1.0f / now : 0.f;
+  // qmax / max|x| is rounded once, 1 / scale of a rounded scale twice: half as many codes on the wrong
+  // side of a tie
+  const float inv = !finite ? 0.f : need == bits ? Q::kMax / __uint_as_float(top) : 1.0f / now;
   if (tid == 0) *scale_at = now;
 
   uint32_t w8[4][2];

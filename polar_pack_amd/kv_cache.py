@@ -118,9 +118,9 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
     For each page and head that gets tokens, k and v apart, in float32::
 
         scale = max(old scale, max|x| / qmax, 2**-64)      qmax 127 (int8) or 448 (e4m3)
-        code  = round(x * (1 / scale))                     ties to even, held to +-qmax
+        code  = round(x * f)                               ties to even, held to +-qmax
 
-    The old scale counts where the page holds earlier tokens of the sequence; where it grows their
+    with f = qmax / max|x| where that sets the scale and 1 / scale otherwise.  The old scale counts where the page holds earlier tokens of the sequence; where it grows their
     codes become ``round(code * (old / scale))``.  A value that is not finite makes its page's scale
     not finite, so that every row that sees the page is NaN.  A page that gets tokens must belong
     to one sequence of the call (shared pages are for tokens already written).

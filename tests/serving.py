@@ -132,13 +132,16 @@ def append(parts, k, v, table, lens, news):
                 c = raw(out[which])[p] if which == 0 else raw(out[which])[p].transpose(1, 2)
                 sc = out[2 + which][p]
                 was = sc.clone() if held else torch.zeros(H)
-                now = torch.maximum(torch.maximum(was, x.abs().amax((1, 2)) / QMAX[dtype]), torch.full((H,), FLOOR))
+                need = x.abs().amax((1, 2)) / QMAX[dtype]
+                now = torch.maximum(torch.maximum(was, need), torch.full((H,), FLOOR))
+                top = torch.full((H,), QMAX[dtype])          # number / tensor would round the reciprocal first
+                factor = torch.where(need == now, top / x.abs().amax((1, 2)), torch.ones(H) / now)
                 for h in range(H):
                     ok = bool(torch.isfinite(now[h]))
                     if held and (not ok or now[h] > was[h]):
                         old = c[h, :held].clone().view(dtype).float() * (was[h] / now[h])
                         c[h, :held] = raw(round_codes(old, dtype)) if ok else 0
-                    c[h, held:held + hi - lo] = raw(round_codes(x[h] * (1.0 / now[h]), dtype)) if ok else 0
+                    c[h, held:held + hi - lo] = raw(round_codes(x[h] * factor[h], dtype)) if ok else 0
                 sc.copy_(now)
         at += n
     return out
