@@ -19,6 +19,17 @@ namespace pp {
 // Scales stay out of the codes: ks multiplies a lane's scores, log2 vs is added to the exponent,
 // so that weights e^(s - m) vs are at most 2^14 in fp16 whatever the scales, and the sum of
 // e^(s - m) takes them times 1 / vs.
+//
+// What bounds it: the codes' way from memory.  A copy that only loads takes as long as the kernel
+// (attend_batch 131.7 against 134.9 us when that was measured).  Four sequences of 100-131 k tokens,
+// 248 MB: 52 us, of which the loads stream for 36 (6.9 TB/s, what any kernel reads here), 5 until
+// the first codes arrive (lengths, pages, codes: three round trips), 3 for a share's sums to be in memory and
+// 5-7 for the join.  64 sequences of 77-8190 tokens, 559 MB: 100 us (5.6 TB/s): a workgroup's 2 shares
+// of row tiles each fill the loads' pipeline anew.  Equal shares against one workgroup a row
+// tile 100 / 124 us; one workgroup a CU with two tiles on their way against two with one 112 / 118
+// (and 65 / 69 at the long sequences, whose join reads half as many parts); a turn counted as 16 tiles
+// against 4 66.4 -> 63.2.  V with the streaming cache policy, since a load takes whole lines of it; not K,
+// whose lines two loads share.
 template <int I>
 using Int = std::integral_constant<int, I>;
 
@@ -362,7 +373,11 @@ __global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A)
   }
 }
 
-// The row tile by the mean rows a sequence and head; a workgroup a CU.
+// The row tile by the mean rows a sequence and head: up to 32 rows the few-row kernel in 16 or 32 (8
+// queries x 2048 tokens of 4 sequences took 182 us on it and take 102 on the many-row kernel, at 33 rows and
+// more the codes are worth converting once), from 129 rows on 256, which 8 wavefronts share.
+// Shares for a workgroup a CU; none for batches that one workgroup cannot count, and none for
+// prompts of two row tiles a CU and more, where cutting row tiles costs more than it evens out.
 static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
                           int64_t q_heads) {
   const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch, cus = device_cu_count();

@@ -45,6 +45,12 @@ def test_single_tokens(H, G, D, bs, codes, value):
     check(H, G, D, bs, codes, value, lens, [1] * len(lens), cu=False)
 
 
+@pytest.mark.parametrize("G,D", [(33, 64), (40, 128), (128, 64), (130, 128)])
+def test_single_tokens_of_wide_groups(G, D):
+    """More query heads a key head than the few-row kernel takes."""
+    check(1, G, D, 64, INT8, F16, [1, 64, 65, 200, 777], [1] * 5, cu=False)
+
+
 @pytest.mark.parametrize("codes,value", [(INT8, F16), (E4M3, BF16)])
 @pytest.mark.parametrize("L", [1023, 1024, 4097, 20000])
 def test_one_long_sequence(L, codes, value):
