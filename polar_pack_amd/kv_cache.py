@@ -37,6 +37,9 @@ class KVCache:
 
     ``k`` codes (pages, heads, block, D) and ``v`` codes (pages, heads, D, block), int8 or
     float8_e4m3fn; ``k_scale`` and ``v_scale`` float32 (pages, heads).  A value is code * scale.
+    Scales are 2**-64 or more (smaller ones count as that in an attention's values) or not finite;
+    codes of tokens before a sequence's length are finite, as :func:`kv_append` writes them: a NaN code put
+    there by other means may reach rows that do not see it.  What lies past the lengths may hold anything.
     :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.
     """
 
@@ -120,8 +123,9 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
         scale = max(old scale, max|x| / qmax, 2**-64)      qmax 127 (int8) or 448 (e4m3)
         code  = round(x * f)                               ties to even, held to +-qmax
 
-    with f = qmax / max|x| where that sets the scale and 1 / scale otherwise.  The old scale counts where the page holds earlier tokens of the sequence; where it grows their
-    codes become ``round(code * (old / scale))``.  A value that is not finite makes its page's scale
+    with f = qmax / max|x| where that sets the scale and 1 / scale otherwise.  The old scale counts
+    where the page holds earlier tokens of the sequence; where it grows their codes become
+    ``round(code * (old / scale))``.  A value that is not finite makes its page's scale
     not finite, so that every row that sees the page is NaN.  A page that gets tokens must belong
     to one sequence of the call (shared pages are for tokens already written).
     """
