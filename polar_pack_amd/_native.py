@@ -6,6 +6,7 @@ The product path has no fallback: if the library is missing or cannot load,
 from __future__ import annotations
 
 import collections
+import contextlib
 import ctypes as C
 import functools
 import os
@@ -214,6 +215,16 @@ def raw_stream(dev) -> int:
     import torch
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(idx)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """``torch.cuda.device(dev)``, or nothing where ``dev`` (with an index) is current already: that
+    context takes 2-3 us, as long as a launch."""
+    import torch
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def packable(ws) -> bool:

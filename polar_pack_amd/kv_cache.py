@@ -136,7 +136,7 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
         raise ValueError("k and v must have one shape and type")
     n = k.shape[0]
     call = _call(cache, block_table, lengths, cu, n)
-    with torch.cuda.device(cache.device):
+    with nat.on_device(cache.device):
         nat.check(nat.lib().pp_kv_append(cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                                          v.stride(0), v.stride(1), _VALUES[k.dtype], n, *call,
                                          nat.raw_stream(cache.device)), "pp_kv_append")
@@ -154,7 +154,7 @@ def kv_read(cache, block_table, lengths, cu=None, *, total=None, dtype=torch.flo
             raise ValueError("total must be given with cu")
         total = block_table.shape[0]
     call = _call(cache, block_table, lengths, cu, total)
-    with torch.cuda.device(cache.device):
+    with nat.on_device(cache.device):
         out = torch.empty((2, total, cache.heads, cache.head_dim), dtype=dtype, device=cache.device)
         k, v = out.unbind(0)
         nat.check(nat.lib().pp_kv_read(cache._ref, *call, total, _READS[dtype], k.data_ptr(), v.data_ptr(),
@@ -183,7 +183,7 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
     call = _call(cache, block_table, lengths, cu, n)
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
     dev = cache.device
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         out = torch.empty((n, heads, cache.head_dim), dtype=q.dtype, device=dev)
         lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
         shape = (dev.index, cache.heads, cache.head_dim, cache.block, call[2], call[5], n, heads)

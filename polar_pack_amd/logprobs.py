@@ -45,7 +45,7 @@ def token_logprobs(logits, tokens, *, top=0):
     per_row = 1 if tokens.dim() == 1 else tokens.shape[1]
     if tokens.dim() == 2 and per_row > 1 and tokens.stride(1) != 1:
         tokens = tokens.contiguous()
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         stats = torch.empty(rows * (per_row + 1 + top), dtype=torch.float32, device=dev)
         lp, entropy, tl = stats.split([rows * per_row, rows, rows * top])
         ids = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
