@@ -28,13 +28,15 @@ namespace pp {
 // of row tiles each fill the loads' pipeline anew.  Equal shares against one workgroup a row
 // tile 100 / 124 us; one workgroup a CU with two tiles on their way against two with one 112 / 118
 // (and 65 / 69 at the long sequences, whose join reads half as many parts); a turn counted as 16 tiles
-// against 4 66.4 -> 63.2.  V with the streaming cache policy, since a load takes whole lines of it; not K,
+// against 4 66.4 -> 63.2.  With 64 values a head a workgroup's registers leave room for a second on the CU, and
+// a tile is half the bytes on its way: 24 sequences of 5 drafted tokens in a window of 2000, 34.5 -> 30.7 us with
+// two.  V with the streaming cache policy, since a load takes whole lines of it; not K,
 // whose lines two loads share.
 template <int I>
 using Int = std::integral_constant<int, I>;
 
 template <int CODES, typename IO, int D, int RT, int NP>
-__global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(const AttnArgs A) {
   constexpr int J = D / 64, DT = D / 16, R = 16 * RT, BUF = D * RT <= 256 ? 2 : 1;
   const KvCache& C = A.C;
   const KvSeqs& S = A.S;
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(256, 1) void kv_attn_split_kernel(const AttnArgs A)
 // The row tile by the mean rows a sequence and head: up to 32 rows the few-row kernel in 16 or 32 (8
 // queries x 2048 tokens of 4 sequences took 182 us on it and take 102 on the many-row kernel, at 33 rows and
 // more the codes are worth converting once), from 129 rows on 256, which 8 wavefronts share.
-// Shares for a workgroup a CU; none for batches that one workgroup cannot count, and none for
+// Shares for a workgroup a CU, two of few rows with 64 values a head (kv_attn_split_kernel); none for batches that one workgroup cannot count, and none for
 // prompts of two row tiles a CU and more, where cutting row tiles costs more than it evens out.
 static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
                           int64_t q_heads) {
@@ -384,7 +386,7 @@ static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width
   AttnPlan P;
   P.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 || D > 128 ? 128 : 256;
   const int64_t row_tiles = tokens * group / P.rows + batch + 1;
-  P.shares = (cus + heads - 1) / heads;
+  P.shares = ((P.rows <= 32 && D == 64 ? 2 : 1) * cus + heads - 1) / heads;
   const int64_t most = row_tiles * ((width * block + 255) / 256 + 1);       // of 4 tiles each
   if (P.shares > most) P.shares = most;
   if (batch > KV_DEAL_BATCH || (P.rows > 32 && tokens * q_heads / P.rows >= 2 * cus)) P.shares = 0;
