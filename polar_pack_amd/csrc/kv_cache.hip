@@ -105,30 +105,28 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
 
   const int tg = tid / (D / 8), dg = tid % (D / 8);    // tokens 4*tg.., values 8*dg..
   const bool mine = tid < (C.block / 4) * (D / 8);
-  float x[4][8];
-  uint32_t top = 0;
+  // Magnitudes of 16-bit values are ordered like their words, NaN last, so the maximum is taken of those.
+  u32x4 x[4];
+  u16x2 big = {0, 0};
   const uint16_t* src = A.x[isv] + (int64_t)head * A.sh[isv];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * tg + i;
-    if (mine && t >= held && t < end) {
-      load8<IO>(src + (P.row0 + t) * A.st[isv] + 8 * dg, A.vec, x[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
-    }
+    x[i] = u32x4{0, 0, 0, 0};
+    if (mine && t >= held && t < end) x[i] = load8(src + (P.row0 + t) * A.st[isv] + 8 * dg, A.vec);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, mag(x[i][j]));
-  top = wave_umax(top);
+    for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, x[i][j] & 0x7fff7fffu));
+  uint32_t top = wave_umax(max((uint32_t)big[0], (uint32_t)big[1]));
   if ((tid & 63) == 0) red[tid >> 6] = top;
   const int64_t ph = (int64_t)P.page * C.heads + head;
   float* scale_at = (isv ? C.vs : C.ks) + ph;
   const float was = held ? *scale_at : 0.f;
   __syncthreads();
   for (int w = 0; w < (nthr + 63) / 64; ++w) top = max(top, red[w]);
+  top = mag(IO::get((uint16_t)top));
   // unsigned order: scales are not negative, and a NaN stays
   const uint32_t need = mag(__uint_as_float(top) / Q::kMax);
   const uint32_t bits = max(need, max(mag(was), mag(KV_SCALE_MIN)));
@@ -145,10 +143,12 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      w8[i][j] = finite ? Q::pack(x[i][4 * j] * inv, x[i][4 * j + 1] * inv, x[i][4 * j + 2] * inv,
-                                  x[i][4 * j + 3] * inv)
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t u = x[i][2 * j], v = x[i][2 * j + 1];
+      w8[i][j] = finite ? Q::pack(IO::get((uint16_t)u) * inv, IO::get((uint16_t)(u >> 16)) * inv,
+                                  IO::get((uint16_t)v) * inv, IO::get((uint16_t)(v >> 16)) * inv)
                         : 0u;
+    }
   auto rescale = [&](uint32_t w) {
     float f[4];
     Q::unpack(w, f);
@@ -175,11 +175,11 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
   const int ld = C.block / 4 + 1;
   if (mine) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t w = 0;
+    for (int j = 0; j < 2; ++j) {
+      uint32_t c[4] = {w8[0][j], w8[1][j], w8[2][j], w8[3][j]};
+      swap_bytes(c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w |= ((w8[i][j / 4] >> (8 * (j & 3))) & 255u) << (8 * i);
-      tile[(8 * dg + j) * ld + tg] = w;
+      for (int i = 0; i < 4; ++i) tile[(8 * dg + 4 * j + i) * ld + tg] = c[i];
     }
   }
   __syncthreads();
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(1024) void kv_read_kernel(const ReadArgs A) {
   extern __shared__ uint32_t tile[];
   const bool none = P.page < 0;                        // read page 0, write zeros
   const int64_t ph = (int64_t)(none ? 0 : P.page) * C.heads + head, base = ph * (C.block * D);
-  const float scale = (isv ? C.vs : C.ks)[ph];
+  const float scale = none ? 0.f : (isv ? C.vs : C.ks)[ph];
   const int tg = tid / (D / 8), dg = tid % (D / 8);
   const bool mine = tid < (C.block / 4) * (D / 8);
   uint32_t w8[4][2];
@@ -238,13 +238,9 @@ __global__ __launch_bounds__(1024) void kv_read_kernel(const ReadArgs A) {
       uint32_t c[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = tile[(8 * dg + 4 * j + i) * ld + tg];
+      swap_bytes(c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w |= ((c[e] >> (8 * i)) & 255u) << (8 * e);
-        w8[i][j] = w;
-      }
+      for (int i = 0; i < 4; ++i) w8[i][j] = c[i];
     }
   } else {
     if (!mine) return;
@@ -262,16 +258,17 @@ __global__ __launch_bounds__(1024) void kv_read_kernel(const ReadArgs A) {
     if (t < P.lo || t >= P.hi) continue;
     raw* o = reinterpret_cast<raw*>(A.out[isv]) + ((P.row0 + t) * C.heads + head) * D + 8 * dg;
     float x[8];
-    Q::unpack(w8[i][0], x);
-    Q::unpack(w8[i][1], x + 4);
-    struct alignas(sizeof(raw) * 4) V4 { raw e[4]; } a, b;
+    Q::unpack(none ? 0u : w8[i][0], x);
+    Q::unpack(none ? 0u : w8[i][1], x + 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a.e[j] = IO::put(none ? 0.f : x[j] * scale);
-      b.e[j] = IO::put(none ? 0.f : x[4 + j] * scale);
+    for (int j = 0; j < 8; ++j) x[j] *= scale;
+    if constexpr (sizeof(raw) == 4) {
+      reinterpret_cast<f32x4*>(o)[0] = f32x4{x[0], x[1], x[2], x[3]};
+      reinterpret_cast<f32x4*>(o)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      *reinterpret_cast<u32x4*>(o) = u32x4{IO::put2(x[0], x[1]), IO::put2(x[2], x[3]), IO::put2(x[4], x[5]),
+                                           IO::put2(x[6], x[7])};
     }
-    reinterpret_cast<V4*>(o)[0] = a;
-    reinterpret_cast<V4*>(o)[1] = b;
   }
 }
 

@@ -14,6 +14,8 @@ namespace pp {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -90,13 +92,13 @@ struct KvCodes;
 template <>
 struct KvCodes<PP_KV_INT8> {
   static constexpr float kMax = 127.f;
+  // Beside 1.5 * 2^23 a float has no bits below 1: the sum is rounded, ties to even, and its last byte is the
+  // code.  Numbers only.
+  static __device__ __forceinline__ uint32_t code(float x) {
+    return __float_as_uint(__builtin_amdgcn_fmed3f(x, -127.f, 127.f) + 12582912.f);
+  }
   static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
-    const float x[4] = {a, b, c, d};
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w |= ((uint32_t)(int)fminf(fmaxf(rintf(x[i]), -127.f), 127.f) & 255u) << (8 * i);
-    return w;
+    return __builtin_amdgcn_perm(code(b), code(a), 0x0c0c0400u) | __builtin_amdgcn_perm(code(d), code(c), 0x04000c0cu);
   }
   static __device__ __forceinline__ void unpack(uint32_t w, float* x) {
 #pragma unroll
@@ -114,7 +116,7 @@ struct KvCodes<PP_KV_INT8> {
 template <>
 struct KvCodes<PP_KV_E4M3> {
   static constexpr float kMax = 448.f;
-  static __device__ __forceinline__ float hold(float x) { return fminf(fmaxf(x, -448.f), 448.f); }
+  static __device__ __forceinline__ float hold(float x) { return __builtin_amdgcn_fmed3f(x, -448.f, 448.f); }
   static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(hold(a), hold(b), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hold(c), hold(d), w, true);
@@ -135,11 +137,17 @@ struct IoF16 {
   typedef uint16_t raw;
   static __device__ __forceinline__ float get(uint16_t u) { return (float)__builtin_bit_cast(f16, u); }
   static __device__ __forceinline__ uint16_t put(float x) { return __builtin_bit_cast(uint16_t, (f16)x); }
+  static __device__ __forceinline__ uint32_t put2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+  }
 };
 struct IoBf16 {
   typedef uint16_t raw;
   static __device__ __forceinline__ float get(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
   static __device__ __forceinline__ uint16_t put(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+  static __device__ __forceinline__ uint32_t put2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+  }
 };
 struct IoF32 {
   typedef float raw;
@@ -147,20 +155,23 @@ struct IoF32 {
   static __device__ __forceinline__ float put(float x) { return x; }
 };
 
-// 8 consecutive 16-bit values as float; `vec`: at a 16-byte boundary.
-template <typename IO>
-__device__ __forceinline__ void load8(const uint16_t* p, bool vec, float* x) {
-  if (vec) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+// 8 consecutive 16-bit values; `vec`: at a 16-byte boundary.
+__device__ __forceinline__ u32x4 load8(const uint16_t* p, bool vec) {
+  if (vec) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = IO::get((uint16_t)w[i]);
-      x[2 * i + 1] = IO::get((uint16_t)(w[i] >> 16));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = IO::get(p[i]);
-  }
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return w;
+}
+
+// Byte i of word j becomes byte j of word i.
+__device__ __forceinline__ void swap_bytes(uint32_t* w) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
 // Host side: the checks every entry point makes of a cache and its sequences.
