@@ -79,7 +79,7 @@ __device__ __forceinline__ int wave_min(int v) {
 }
 __device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
 
-// Work item `at` of the call: tiles of R rows, sequence after sequence.
+// Work item `at` of the call: tiles of R rows (a power of two), sequence after sequence.
 __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, RowTile& T) {
   if (A.S.cu == nullptr) {
     const int per = (A.group + R - 1) / R;
@@ -87,8 +87,8 @@ __device__ __forceinline__ bool kv_row_tile(const AttnArgs& A, int at, int R, Ro
     if (T.b >= A.S.batch) return false;
     T.r0 = (at - T.b * per) * R;
   } else {
-    T.b = kv_find(A.S, at, A.group, R, 1);
-    T.r0 = (at - kv_begin(A.S, T.b, A.group, R, 1)) * R;
+    T.b = kv_find(A.S, at, A.group, __builtin_ctz(R), 1);
+    T.r0 = (at - kv_begin(A.S, T.b, A.group, __builtin_ctz(R), 1)) * R;
   }
   T.b = uniform(T.b);
   return kv_tile_fill(A, R, T);

@@ -61,8 +61,8 @@ struct Piece {
 __device__ __forceinline__ bool kv_piece(const KvCache& C, const KvSeqs& S, int at, Piece& P) {
   int b = at, slot = 0;
   if (S.cu != nullptr) {
-    b = kv_find(S, at, 1, C.block, 2);
-    slot = at - kv_begin(S, b, 1, C.block, 2);
+    b = kv_find(S, at, 1, C.shift, 2);
+    slot = at - kv_begin(S, b, 1, C.shift, 2);
   }
   const int s0 = kv_start(S, b), n = kv_start(S, b + 1) - s0;
   if (n <= 0) return false;

@@ -52,19 +52,19 @@ __device__ __forceinline__ int kv_start(const KvSeqs& S, int b) {
 }
 
 // The sequence whose work items hold item `at`, where sequence b's begin at
-// floor(start(b) * mul / rows) + slack * b: the last b in [0, batch] that begins at or before `at`.
+// (start(b) * mul >> shift) + slack * b: the last b in [0, batch] that begins at or before `at`.
 // A wavefront looks at 64 sequences a step.  Every wavefront of the workgroup calls it.
-__device__ __forceinline__ int kv_begin(const KvSeqs& S, int b, int mul, int rows, int slack) {
-  return (int)((int64_t)kv_start(S, b) * mul / rows) + slack * b;
+__device__ __forceinline__ int kv_begin(const KvSeqs& S, int b, int mul, int shift, int slack) {
+  return (int)((int64_t)kv_start(S, b) * mul >> shift) + slack * b;
 }
 
-__device__ __forceinline__ int kv_find(const KvSeqs& S, int at, int mul, int rows, int slack) {
+__device__ __forceinline__ int kv_find(const KvSeqs& S, int at, int mul, int shift, int slack) {
   const int lane = threadIdx.x & 63;
   int lo = 0, span = S.batch + 1;            // the answer is in [lo, lo + span)
   while (span > 1) {
     const int step = (span + 63) / 64;
     const int b = lo + lane * step;
-    const bool ok = b < lo + span && kv_begin(S, b, mul, rows, slack) <= at;
+    const bool ok = b < lo + span && kv_begin(S, b, mul, shift, slack) <= at;
     const uint64_t mask = __ballot(ok || lane == 0);
     const int last = 63 - __builtin_clzll(mask);
     const int end = lo + span;
