@@ -1,7 +1,7 @@
 """Four packed models answer a prompt in lock step: packed Linears, the 8-bit cache, its attention and
 the log probabilities of what is chosen.
 
-    python examples/decode_four_models.py
+    python -m examples.decode_four_models       (from the root of the repository)
 
 A one-layer decoder of random weights stands for each model.  Its Linears come from one
 quad stream; the four models' rows go through a Linear together, each keeping its own model's
