@@ -185,6 +185,14 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
   __syncthreads();
   uint32_t* v = reinterpret_cast<uint32_t*>(C.v + base);
   const int wl = C.shift - 2, words = D << wl;
+  if (held == 0 && end == C.block) {                   // all new: whole 16-byte pieces
+    const int ql = wl - 2;
+    for (int w = tid; w < D << ql; w += nthr) {
+      const uint32_t* t = tile + (w >> ql) * ld + 4 * (w & ((1 << ql) - 1));
+      reinterpret_cast<u32x4*>(v)[w] = u32x4{t[0], t[1], t[2], t[3]};
+    }
+    return;
+  }
   for (int w = tid; w < words; w += nthr) {
     const int d = w >> wl, g = w & ((1 << wl) - 1), t0 = 4 * g;
     if (t0 >= end || (t0 + 4 <= held && !grown)) continue;
@@ -228,9 +236,14 @@ __global__ __launch_bounds__(1024) void kv_read_kernel(const ReadArgs A) {
   const bool mine = tid < (C.block / 4) * (D / 8);
   uint32_t w8[4][2];
   if (isv) {
-    const uint32_t* v = reinterpret_cast<const uint32_t*>(C.v + base);
-    const int wl = C.shift - 2, ld = C.block / 4 + 1;
-    for (int w = tid; w < (D << wl); w += nthr) tile[(w >> wl) * ld + (w & ((1 << wl) - 1))] = v[w];
+    const u32x4* v = reinterpret_cast<const u32x4*>(C.v + base);
+    const int ql = C.shift - 4, ld = C.block / 4 + 1;
+    for (int w = tid; w < D << ql; w += nthr) {
+      const u32x4 c = v[w];
+      uint32_t* t = tile + (w >> ql) * ld + 4 * (w & ((1 << ql) - 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = c[i];
+    }
     __syncthreads();
     if (!mine) return;
 #pragma unroll
