@@ -126,9 +126,8 @@ struct KvCodes<PP_KV_E4M3> {
     hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
   }
   static __device__ __forceinline__ void unpack(uint32_t w, float* x) {
-    f16x2 lo, hi;
-    halves(w, lo, hi);
-    x[0] = (float)lo[0]; x[1] = (float)lo[1]; x[2] = (float)hi[0]; x[3] = (float)hi[1];
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = lo[0]; x[1] = lo[1]; x[2] = hi[0]; x[3] = hi[1];
   }
 };
 
