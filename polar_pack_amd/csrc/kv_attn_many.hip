@@ -77,6 +77,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
   } else {
     U.at = U.end;
   }
+  // The same in every lane, and said so: what is asked of them becomes a branch then, and no lanes are switched off.
+  // Where they were, hipcc 7.2 saved registers at the join before it switched the lanes on again, and loaded back
+  // garbage (192 and 256 values a head in pages of 32, writes through such addresses; tests/test_device_code.py).
+  a = uniform(a);
+  z = uniform(z);
+  T.lim = uniform(T.lim);
 
   // this lane's row: column m32 of the wavefront's row tile
   f16x8 q[KS];

@@ -72,6 +72,15 @@ def test_prompts(H, G, D, bs, codes, value):
     check(H, G, D, bs, codes, value, lens, news)
 
 
+@pytest.mark.parametrize("codes,value", [(INT8, F16), (INT8, BF16), (E4M3, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("D", [192, 256])
+@pytest.mark.parametrize("bs", [16, 32])
+def test_prompts_of_wide_heads_in_small_pages(bs, D, codes, value):
+    """Where the many-row kernel has the fewest registers to spare; several row tiles a workgroup."""
+    check(2, 2, D, bs, codes, value, [450, 150, 40], [150, 150, 30])
+    check(1, 2, D, bs, codes, value, [450, 150, 40], [150, 150, 30], causal=False)
+
+
 @pytest.mark.parametrize("G", [1, 8])
 def test_prompt_piece_behind_a_long_prefix(G):
     check(1, G, 128, 64, INT8, F16, [5003], [150])
