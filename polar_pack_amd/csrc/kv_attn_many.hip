@@ -289,7 +289,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
     read_k(Int<0>(), kl, 0);
     scores(kl);
     weigh(sc);
-    if (PING && wave >= WAVES / 2) phase();
+    // The rings: beside the weights of tile i, V of tile i + 1 and K of tile i + 2 are written over what the products of
+    // an earlier step read last, with a barrier between them.  K of the first tile is read just above instead, and
+    // with two slots the first tile's weights already write over it: so a barrier here.  With three slots the
+    // second tile's do; there the barrier is the one by which the second four run behind.
+    if (!PING || wave >= WAVES / 2) phase();
     int r0 = 0;                                               // ring of V of tile i, and of K
     for (int i = a; i < z; ++i) {
       const int t0 = i * 64, r1 = r0 + 1 == RING ? 0 : r0 + 1, r2 = r1 + 1 == RING ? 0 : r1 + 1;

@@ -228,6 +228,45 @@ def test_many_row_tiles(B, n):
     check(1, 32, 64, 64, INT8, BF16, [m + 30 * (i % 3) for i, m in enumerate(news)], news, extra=3)
 
 
+@pytest.mark.parametrize("codes,value", [(INT8, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("H,G,D,bs,kw", [(1, 2, 192, 64, {}), (2, 4, 256, 64, {}), (1, 2, 256, 16, {"window": 90}),
+                                         (1, 4, 192, 32, {"causal": False}), (2, 2, 128, 128, {}),
+                                         (1, 3, 64, 16, {"window": 70})])
+def test_row_tiles_of_four_wavefronts(H, G, D, bs, kw, codes, value):
+    """At 33-128 rows a sequence and head, and at 192 and 256 values a head whatever the rows, a workgroup is 4
+    wavefronts and its ring of keys has two slots: each wavefront has read the first tile of keys before any
+    writes the third over it.  Prompts of one to eight tiles, several row tiles a workgroup."""
+    n = 20 if D <= 128 else 150
+    lens, news = [n + 300, n, n + 30, 3 * n + 64, n + 1], [n, n, n - 3, n + 5, 1]
+    check(H, G, D, bs, codes, value, lens, news, **kw)
+
+
+@pytest.mark.parametrize("codes,value,D,window", [(INT8, F16, 256, 0), (E4M3, BF16, 192, 40), (E4M3, F16, 128, 0)])
+def test_many_row_tiles_of_four_wavefronts(codes, value, D, window):
+    """The same with row tiles enough for every CU, which are not shared; 96-124 rows a sequence and head at 128
+    values a head."""
+    B, n, G = (170, 3, 32) if D == 128 else (21, 25, 32)
+    H = 4
+    g = torch.Generator().manual_seed(D)
+    news = torch.randint(n, n + 2, (B,), generator=g).tolist()
+    while sum(news) * H * G / 128 < 2 * torch.cuda.get_device_properties(DEV).multi_processor_count:
+        news = [x + 1 for x in news]
+    check(H, G, D, 64, codes, value, [m + 60 * (i % 3) for i, m in enumerate(news)], news, window=window, extra=2)
+
+
+@pytest.mark.parametrize("G,D,news", [(4, 64, [20, 25]), (4, 256, [150, 90]), (8, 128, [150, 90])])
+def test_one_answer_of_many_rows(G, D, news):
+    g = torch.Generator().manual_seed(D)
+    parts = random_cache(110, 2, 64, D, INT8, g)
+    lens = [5000, 777]
+    table = tables(lens, 64, 110, g).to(DEV)
+    cache, L, cu = device_cache(parts), torch.tensor(lens, dtype=torch.int32, device=DEV), offsets(news).to(DEV)
+    q = torch.randn(sum(news), 2 * G, D, generator=g).half().to(DEV)
+    want = kv_attention(q, cache, table, L, cu)
+    for _ in range(5):
+        assert torch.equal(kv_attention(q, cache, table, L, cu), want)
+
+
 def test_one_answer():
     """Joins do not depend on the order in which parts of a row end."""
     g = torch.Generator().manual_seed(3)
