@@ -5,9 +5,14 @@
 
 namespace pp {
 
-// Weights e^(s - m) vs are kept up to 2^14 in fp16: the smallest that is not flushed is 2^-38 of the
-// largest.
+// Weights are 2^(s - ref), s with log2 of vs in it, ref 14 below the largest s: up to 2^14 in fp16, the smallest that is
+// not flushed 2^-38 of the largest.  Past 2^24 floats are so far apart that the 14 would round to 16, whose 2^16 fp16
+// does not hold; ref is the largest s itself there.
 constexpr float KV_P_LOG2 = 14.f;
+__device__ __forceinline__ float kv_ref(float top) {
+  const float ref = top - KV_P_LOG2;
+  return top - ref > 15.f ? top : ref;
+}
 
 // A row tile of many rows whose keys several workgroups share: the parts, and the rows.
 struct ManyPart {
@@ -22,7 +27,7 @@ struct AttnArgs {
   uint16_t* out;
   float* lse;
   float* parts;     // [head][workgroup][2][row][D + 4]: what a workgroup has of a row tile that it shares: sums of
-                    // values, maximum, sum of weights; 1: of the one that begins in it, 0: of one that began before
+                    // values, reference, sum of weights; 1: of the one that begins in it, 0: of one that began before
   ManyPart* desc;   // [head][workgroup] (many rows): the shared row tile that begins in it, runs 0: none
   uint32_t* counts; // [head][workgroup]: parts that are done of the row tile that begins in it; 0 before and after
   int q_heads, group, window, causal, q_vec;
@@ -365,7 +370,7 @@ __device__ __forceinline__ float many_q(const AttnArgs& A, int token, int hq, in
   return scale_q<IO, D / 16, 32>(A, w, q);
 }
 
-// (m, l, v) takes the part (mp, lp, w), both sums of e^(s - their maximum).
+// (m, l, v) takes the part (mp, lp, w), both sums of 2^(s - their reference).
 template <int W>
 __device__ __forceinline__ void join_part(float& m, float& l, float* v, float mp, float lp, const float* w) {
   const float mn = fmaxf(m, mp);
@@ -379,8 +384,8 @@ __device__ __forceinline__ void join_part(float& m, float& l, float* v, float mp
 
 // 1 / l, and 0 for a row that saw nothing; a NaN stays.
 __device__ __forceinline__ float kv_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
-__device__ __forceinline__ float kv_lse(float m, float l) {
-  return l == 0.f ? -INFINITY : (m - KV_P_LOG2 + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+__device__ __forceinline__ float kv_lse(float ref, float l) {
+  return l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 template <typename IO>

@@ -196,15 +196,16 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
 #pragma unroll
       for (int k = 0; k < 16; ++k) top = fmaxf(top, e[k]);
       top = max_groups(top);
-      if (__any(top > mx[x])) {
-        const float mn = fmaxf(mx[x], top);
+      const float next = kv_ref(top);
+      if (__any(next > mx[x])) {
+        const float mn = fmaxf(mx[x], next);
         const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[x] - mn);
         mx[x] = mn;
         l[x] *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[x][d] *= f;
       }
-      const float ref = (mx[x] == -INFINITY ? 0.f : mx[x]) - KV_P_LOG2;
+      const float ref = mx[x] == -INFINITY ? 0.f : mx[x];
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {

@@ -33,7 +33,7 @@ using Int = std::integral_constant<int, I>;
 
 typedef const __attribute__((address_space(1))) u32x4* GlobalCodes;    // not a flat address, whose loads wait for LDS
 
-constexpr float KV_NONE = -1e30f, KV_NEAR = 12.f, KV_FAR = 65000.f;
+constexpr float KV_NONE = -3.40282347e38f, KV_NEAR = 12.f, KV_FAR = 65000.f;   // no reference yet: no score is less
 
 template <int CODES, typename IO, int D, int WAVES, int NP>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(const AttnArgs A) {
@@ -340,13 +340,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
         const bool need = (ref == KV_NONE) | (max_halves(most) > KV_FAR);
         const float next = need ? fmaxf(ref, max_halves(top) + from - KV_NEAR) : ref;
         const float f = __builtin_amdgcn_exp2f(ref - next);
+        // 12 is the most that a row's new exponents are, but past 2^24, where the floats around the reference are 8
+        // and more apart: what passes 15 there is 15, whose weight fp16 holds
+        const float hold = need ? 15.f : INFINITY;
         l *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[0][e] += from - next;
-          s[1][e] += from - next;
+          const float x = s[0][e] + (from - next), y = s[1][e] + (from - next);
+          s[0][e] = x > hold ? hold : x;
+          s[1][e] = y > hold ? hold : y;
         }
         ref = next;
         weights();
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
         for (int k = 0; k < 4; ++k)
           store4<IO>(A.out + at * D + 32 * d + 8 * k + 4 * hh,
                      f32x4{o[d][4 * k] * inv, o[d][4 * k + 1] * inv, o[d][4 * k + 2] * inv, o[d][4 * k + 3] * inv});
-      if (A.lse && hh == 0) A.lse[at] = kv_lse(ref + KV_P_LOG2, l);
+      if (A.lse && hh == 0) A.lse[at] = kv_lse(ref, l);
     } else {
       // workgroup owner + i has part i; the owner's is its second
       float* part = A.parts + (((int64_t)h * A.shares + blockIdx.x) * 2 + (run == 0)) * R * (D + 4) + (int64_t)rr * (D + 4);
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
           *reinterpret_cast<f32x4*>(part + 32 * d + 8 * k + 4 * hh) =
               f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
       if (hh == 0) {
-        part[D] = ref + KV_P_LOG2;
+        part[D] = ref;
         part[D + 1] = l;
       }
     }

@@ -152,6 +152,49 @@ def test_queries_of_any_size(value, q_scale, many):
     check(1, 8, 128, 64, INT8, value, [300], [many], q_scale=q_scale, scale=0.0)
 
 
+def one_score(codes, size, keys, many, marked=None):
+    """Attention of ``many`` tokens, the last of ``keys``, to keys that all have the score ``size`` (base 2), except
+    that with ``marked`` all but that one have -``size``; and the values."""
+    g = torch.Generator().manual_seed(keys + many)
+    parts = random_cache(-(-keys // 64), 1, 64, 64, codes, g)
+    parts[0].copy_((torch.full(parts[0].shape, 100.0 if marked is None else -100.0)).to(codes))
+    if marked is not None:
+        parts[0][marked // 64, 0, marked % 64] = torch.full((64,), 100.0).to(codes)
+    for t in parts[2:]:
+        t.fill_(2.0 ** -6)
+    table = torch.arange(-(-keys // 64), dtype=torch.int32)[None]
+    q = torch.ones(many, 4, 64, dtype=torch.float16)
+    code = float(parts[0].double().abs().max())
+    got, lse = kv_attention(q.to(DEV), device_cache(parts), table.to(DEV),
+                            torch.tensor([keys], dtype=torch.int32, device=DEV), offsets([many]).to(DEV),
+                            scale=size * math.log(2) / (code * 64 * 2.0 ** -6), return_lse=True)
+    values = parts[1][:, 0].double().transpose(1, 2).reshape(-1, 64) * 2.0 ** -6
+    return got.cpu().double(), lse.cpu().double(), values
+
+
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("many", [1, 12, 150])
+@pytest.mark.parametrize("size", [2.0 ** e * f for e in (23, 24, 25, 26, 27, 28, 40) for f in (1.01, 1.3, 1.9)])
+def test_scores_that_are_large(size, many, codes):
+    """Where neighbouring floats are 1 to 16 apart, and beyond: weights are still at most what fp16 holds, and the
+    key that is ahead has all of it."""
+    got, lse, values = one_score(codes, size, 300, many, marked=70)
+    assert ((got - values[70]).abs() <= 2.0 ** -11 * values[70].abs()).all()
+    assert ((lse - size * math.log(2)).abs() <= 2.0 ** -20 * size).all()
+
+
+@pytest.mark.parametrize("many", [1, 12, 60])
+@pytest.mark.parametrize("size", [-1e29, -1e31, -3e37, 1e31])
+def test_scores_as_large_as_floats(size, many):
+    """A row whose scores are all far below zero sees its keys all the same."""
+    got, lse, values = one_score(INT8, size, 64, many)
+    for i in range(many):
+        seen = values[:64 - many + 1 + i]
+        want, mass = seen.mean(0), seen.abs().mean(0)
+        assert ((got[i] - want).abs() <= 2.0 ** -11 * (want.abs() + mass) + 2.0 ** -20 * mass).all()
+    assert ((lse - size * math.log(2)).abs() <= 2.0 ** -20 * abs(size)).all()
+
+
 @pytest.mark.parametrize("many", [1, 150])
 def test_queries_that_are_not_finite(many):
     def edit(parts, table, q):
