@@ -337,20 +337,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void kv_attn_many_kernel(con
         float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+        top = max_halves(top);
         const bool need = (ref == KV_NONE) | (max_halves(most) > KV_FAR);
-        const float next = need ? fmaxf(ref, max_halves(top) + from - KV_NEAR) : ref;
+        const float next = need ? fmaxf(ref, top + from - KV_NEAR) : ref;
         const float f = __builtin_amdgcn_exp2f(ref - next);
-        // 12 is the most that a row's new exponents are, but past 2^24, where the floats around the reference are 8
-        // and more apart: what passes 15 there is 15, whose weight fp16 holds
-        const float hold = need ? 15.f : INFINITY;
+        // Past 2^24 the reference is rounded so far that the largest exponent can be 16 and more, whose weight fp16
+        // does not hold: it is 0 there.
+        const float to = (need && top + (from - next) > 15.f) ? -top : from - next;
         l *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = s[0][e] + (from - next), y = s[1][e] + (from - next);
-          s[0][e] = x > hold ? hold : x;
-          s[1][e] = y > hold ? hold : y;
+          s[0][e] += to;
+          s[1][e] += to;
         }
         ref = next;
         weights();
