@@ -57,8 +57,8 @@ class KVCache:
         ts = (k, v, k_scale, v_scale)
         if k.device.type != "cuda" or any(t.device != k.device for t in ts):
             raise ValueError("a cache's tensors must be on one ROCm device")
-        if not all(t.is_contiguous() for t in ts):
-            raise ValueError("a cache's tensors must be contiguous")
+        if not all(t.is_contiguous() and not t.is_neg() for t in ts):
+            raise ValueError("a cache's tensors must be contiguous and hold their values as they are")
         if pages < 1 or heads < 1 or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("a cache needs a page and a head, and codes at 16-byte boundaries")
         self.k, self.v, self.k_scale, self.v_scale = ts
@@ -112,6 +112,8 @@ def _values(cache, x, name, heads):
         raise ValueError(f"{name} must be (tokens, {heads if heads else 'heads'}, {cache.head_dim})")
     if x.device != cache.device:
         raise ValueError("all operands must be on the cache's device")
+    if x.is_neg():                                   # memory that holds the values negated
+        x = x.resolve_neg()
     return x if x.stride(2) == 1 else x.contiguous()
 
 

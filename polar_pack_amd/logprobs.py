@@ -40,6 +40,8 @@ def token_logprobs(logits, tokens, *, top=0):
         raise ValueError("a row needs a logit")
     if not 0 <= top <= min(TOP_MAX, V):
         raise ValueError(f"top must be in 0..{min(TOP_MAX, V)}")
+    if logits.is_neg():                              # memory that holds the values negated
+        logits = logits.resolve_neg()
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     per_row = 1 if tokens.dim() == 1 else tokens.shape[1]

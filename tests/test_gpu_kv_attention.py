@@ -236,6 +236,19 @@ def test_strides_of_queries():
         assert (again.float() - want.float()).abs().max() <= 2.0 ** -9 * want.float().abs().max()
 
 
+def test_queries_that_negate_when_they_are_read():
+    g = torch.Generator().manual_seed(15)
+    parts = random_cache(12, 2, 64, 64, INT8, g)
+    cache = device_cache(parts)
+    for news in ([1, 1], [100, 30]):
+        table, L = tables([300, 200], 64, 12, g).to(DEV), torch.tensor([300, 200], dtype=torch.int32, device=DEV)
+        q = torch.randn(sum(news), 8, 64, generator=g).half().to(DEV)
+        view = torch._neg_view(-q)
+        assert view.is_neg() and torch.equal(view, q)
+        args = (cache, table, L, offsets(news).to(DEV))
+        assert torch.equal(kv_attention(view, *args), kv_attention(q, *args))
+
+
 def test_shared_pages():
     """Two sequences with one prefix: the same rows."""
     g = torch.Generator().manual_seed(6)

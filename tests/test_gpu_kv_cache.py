@@ -227,6 +227,24 @@ def test_append_and_read_in_a_graph_and_on_another_stream():
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
 
 
+def negated(x):
+    """A dense view of ``x``'s values whose memory holds -x."""
+    y = torch._neg_view(-x)
+    assert y.is_neg() and y.stride() == x.stride() and torch.equal(y, x)
+    return y
+
+
+def test_views_that_negate():
+    lens, news = [20, 33], [20, 7]
+    parts, table, k, v = problem(2, 64, 16, torch.int8, lens, news, 37)
+    want = append(parts, k, v, table, lens, news)
+    same(call(parts, table, negated(k.to(DEV)), negated(v.to(DEV)), lens, news), want)
+    same(call(parts, table, k, negated(v.to(DEV)), lens, news), want)
+    on = [t.to(DEV) for t in parts]
+    with pytest.raises(ValueError):
+        KVCache(on[0], on[1], torch._neg_view(on[2]), on[3])
+
+
 def test_refusals():
     g = torch.Generator().manual_seed(0)
     parts = [t.to(DEV) for t in random_cache(2, 2, 16, 64, torch.int8, g)]

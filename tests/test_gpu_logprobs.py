@@ -116,6 +116,17 @@ def test_strides_and_alignment(dtype):
     check(x.t().contiguous().to(DEV).t(), t, 5)
 
 
+def test_logits_that_negate_when_they_are_read():
+    for dtype in (torch.float16, torch.float32):
+        x, t = logits(5, 3001, dtype, 6)
+        x = x.to(DEV)
+        view = torch._neg_view(-x)
+        assert view.is_neg() and torch.equal(view, x)
+        check(view, t, 3)
+        for a, b in zip(token_logprobs(view, t.to(DEV), top=3), token_logprobs(x, t.to(DEV), top=3)):
+            assert torch.equal(a, b)
+
+
 def test_no_rows():
     r = token_logprobs(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV), top=3)
     assert r.logprob.shape == (0,) and r.entropy.shape == (0,) and r.top_ids.shape == (0, 3)
