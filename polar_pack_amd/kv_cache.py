@@ -15,6 +15,9 @@ each sequence's tokens among the call's (None: one token each).  They stay on th
 here waits for it, and every call can be captured in a HIP graph.  What the three tensors hold is
 held to its range on the device: a page outside the cache, or a token past the table, is not
 written, reads zero and is attended by no row.
+
+They serve: none has a backward pass, and what they return carries no gradient, whether their
+arguments ask for one or not.
 """
 from __future__ import annotations
 

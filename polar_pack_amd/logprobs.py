@@ -26,7 +26,8 @@ def token_logprobs(logits, tokens, *, top=0):
     ``tokens`` int64 (rows,) or (rows, n): ``logprob = x[token] - log sum e^x``, NaN for a token outside
     [0, V).  ``entropy = log sum e^x - sum p x``.  ``top`` (at most 64): the largest logits in order,
     equal ones by the lower index.  A logit of -inf has probability 0; a row of nothing else, or one
-    that holds a NaN or +inf, gives NaN.  Sums are held in float32.
+    that holds a NaN or +inf, gives NaN.  Sums are held in float32.  There is no backward pass: the results
+    carry no gradient, whether ``logits`` asks for one or not.
     """
     if logits.dim() != 2 or logits.dtype not in _LOGITS:
         raise TypeError("logits must be float16, bfloat16 or float32 (rows, V)")
