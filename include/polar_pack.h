@@ -793,7 +793,8 @@ int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_t table_ld,
 /*
  * Attention of a call's tokens to the cache.  Query head hq reads head hq / (q_heads / heads).  The row
  * of the call's i-th token of sequence b has position p = lengths[b] - n_b + i and sees the keys of
- * (p - window, p] (causal; window 0: of [0, p]), or all of [0, lengths[b]) (causal 0):
+ * (p - window, p] (causal; window 0: of [0, p]), or all of [0, lengths[b]) (causal 0); causal or not, a row
+ * with p < 0, where a sequence has more of the call's tokens than lengths[b], sees none:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
  * A row that sees no key gives zeros and lse -inf.  q is (tokens, q_heads, head_dim) with strides q_st,
  * q_sh (PP_F16 or PP_BF16), out dense of the same type at a 16-byte boundary, lse null or (tokens,

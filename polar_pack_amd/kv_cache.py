@@ -172,8 +172,11 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
 
     Query head ``hq`` reads head ``hq // (q_heads // heads)``.  The call's i-th token of sequence b has
     position ``p = lengths[b] - n_b + i`` and sees the keys of ``[0, p]``, with ``window > 0`` only the
-    last ``window`` of them, with ``causal=False`` all ``lengths[b]``.  ``scale`` defaults to
-    ``D ** -0.5``.  A row that sees no key is zero (lse -inf).
+    last ``window`` of them, with ``causal=False`` all ``lengths[b]``.  Causal or not, the call's tokens are
+    the last ones of their sequence: one whose position is negative, where a sequence has more queries than
+    ``lengths[b]``, is no token of it and sees nothing (as it is not written and reads zero).  Queries that are
+    not the sequence's own, as in attention to another text, are passed at most ``lengths[b]`` a call.
+    ``scale`` defaults to ``D ** -0.5``.  A row that sees no key is zero (lse -inf).
 
     Returns (tokens, q_heads, D) of q's type, and with ``return_lse`` also the float32 (tokens,
     q_heads) natural logarithms of the sums, by which attention over several caches is joined.

@@ -97,6 +97,25 @@ def test_every_key(news):
     check(2, 4, 128, 32, E4M3, F16, [300, 201, 90], news, causal=False)
 
 
+@pytest.mark.parametrize("G,piece", [(4, 40), (1, 20), (4, 3)])
+def test_queries_of_another_text(G, piece):
+    """150 queries to 40 keys: in calls of at most 40 each sees them all; in one call only the last 40 have a
+    position, and the others see nothing."""
+    g = torch.Generator().manual_seed(piece)
+    parts = random_cache(3, 1, 16, 64, INT8, g)
+    table = tables([40], 16, 3, g)
+    q = torch.randn(150, G, 64, generator=g).half()
+    cache, at = device_cache(parts), (table.to(DEV), torch.tensor([40], dtype=torch.int32, device=DEV))
+    want, tol = (torch.cat(x) for x in zip(*[attention(q[i:i + 40], parts, table, [40], [len(q[i:i + 40])], False)[::2]
+                                             for i in range(0, 150, 40)]))
+    got = torch.cat([kv_attention(x.to(DEV), cache, *at, offsets([len(x)]).to(DEV), causal=False)
+                     for x in q.split(piece)]).cpu().double()
+    assert ((got - want).abs() <= tol).all()
+    whole, lse = kv_attention(q.to(DEV), cache, *at, offsets([150]).to(DEV), causal=False, return_lse=True)
+    assert ((whole[110:].cpu().double() - want[110:]).abs() <= tol[110:]).all()
+    assert not whole[:110].any() and (lse[:110] == -math.inf).all() and lse[110:].isfinite().all()
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("many", [1, 30])
 def test_rows_that_see_nothing(causal, many):
