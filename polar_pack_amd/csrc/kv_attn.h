@@ -305,9 +305,10 @@ __device__ __forceinline__ void to_halves(u32x4 w, f16x8& a, f16x8& b) {
 
 // A row's query as the second operand of S^T = K Q^T: lane group g holds values 64 j + 16 g + 8 e + 0..7
 // as q[j][e], scaled by a power of two so that the largest lies in [2^13, 2^14): bf16 queries of any
-// size keep all their bits in fp16 (what is below 2^-37 of the largest loses some).  load_q issues the
-// loads, make_q returns the factor of the row's sums, score scale and power of two; NaN for a row that
-// is not finite.
+// size fit in fp16 then.  With fp16's smallest step 2^-24 a bf16 value keeps all its bits down to 2^-30 of
+// the row's largest (an fp16 one to 2^-27); smaller ones lose some, and what is below 2^-38 of it is zero.
+// load_q issues the loads, make_q returns the factor of the row's sums, score scale and power of two; NaN for a
+// row that is not finite.
 template <int D>
 __device__ __forceinline__ void load_q(const AttnArgs& A, int token, int hq, int g, bool real, u32x4 (*w)[2]) {
   const uint16_t* p = A.q + (int64_t)token * A.q_st + (int64_t)hq * A.q_sh + 16 * g;

@@ -8,8 +8,9 @@
 namespace pp {
 
 // Few rows a sequence and head (single tokens, drafts).  A workgroup takes 16 * RT rows of one
-// sequence and key/value head and a run of 64-token tiles, dealt to its 4 wavefronts in turn; runs of
-// one row tile are joined by kv_attn_join_kernel.
+// sequence and key/value head and a run of 64-token tiles, dealt to its 4 wavefronts in turn.  Where a row
+// tile has several runs, each leaves its sums in the workspace and counts itself done; the one that
+// counts last reads them all in their order, writes the rows and sets the count back to zero.
 //
 // The codes go from memory to the matrix cores without LDS: S^T = K Q^T takes rows of K as they lie
 // (16 bytes a lane), O^T = V^T P^T rows of the transposed V.  Which token is which row of a product is

@@ -171,6 +171,17 @@ def test_queries_of_any_size(value, q_scale, many):
     check(1, 8, 128, 64, INT8, value, [300], [many], q_scale=q_scale, scale=0.0)
 
 
+@pytest.mark.parametrize("many", [1, 150])
+@pytest.mark.parametrize("value,small", [(BF16, -12), (BF16, -29), (F16, -9)])
+def test_queries_of_unequal_channels(value, small, many):
+    """Channels of 2^small beside one of 1, whose keys are zero: the scores are the small ones', all their bits."""
+    def edit(parts, table, q):
+        parts[0][..., 0] = 0
+        q.clamp_(-1, 1).mul_(2.0 ** small)
+        q[..., 0] = 1
+    check(1, 8, 128, 64, INT8, value, [300], [many], edit=edit, scale=2.0 ** -small / 8)
+
+
 def one_score(codes, size, keys, many, marked=None):
     """Attention of ``many`` tokens, the last of ``keys``, to keys that all have the score ``size`` (base 2), except
     that with ``marked`` all but that one have -``size``; and the values."""
