@@ -172,12 +172,13 @@ def test_queries_of_any_size(value, q_scale, many):
 
 
 @pytest.mark.parametrize("many", [1, 150])
-@pytest.mark.parametrize("value,small", [(BF16, -12), (BF16, -29), (F16, -9)])
+@pytest.mark.parametrize("value,small", [(BF16, -12), (BF16, -30), (F16, -9)])
 def test_queries_of_unequal_channels(value, small, many):
-    """Channels of 2^small beside one of 1, whose keys are zero: the scores are the small ones', all their bits."""
+    """Channels of 2^small to 2^(small + 1) beside one of 1, whose keys are zero: the scores are the small ones', and
+    to 2^-30 of the largest they keep all their bits."""
     def edit(parts, table, q):
         parts[0][..., 0] = 0
-        q.clamp_(-1, 1).mul_(2.0 ** small)
+        q.copy_(torch.copysign(q.abs() % 1 + 1, q) * 2.0 ** small)
         q[..., 0] = 1
     check(1, 8, 128, 64, INT8, value, [300], [many], edit=edit, scale=2.0 ** -small / 8)
 
