@@ -377,16 +377,30 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
   }
 }
 
-// The row tile by the mean rows a sequence and head: up to 32 rows the few-row kernel in 16 or 32 (8
-// queries x 2048 tokens of 4 sequences took 182 us on it and take 102 on the many-row kernel, at 33 rows and
-// more the codes are worth converting once), from 129 rows on 256, which 8 wavefronts share.
-// Shares for a workgroup a CU, two of few rows with 64 values a head (kv_attn_split_kernel); none for batches that one workgroup cannot count, and none for
-// prompts of two row tiles a CU and more, where cutting row tiles costs more than it evens out.
+// The row tile by the mean rows of a sequence and head (tokens x query heads a key head), in us on both sides,
+// sequences of int8 codes of 16 query and 2 key heads of 128 unless said:
+// * 16 or 32 rows at 24: 4 sequences of 4000 tokens 17.6 / 24.4, 64 of 8000 90 / 65.  From 17 rows on 32, which a
+//   large batch reads its codes once for.
+// * 32 rows or the many-row kernel's 128: at 48 rows 4 of 40,000 50 / 67, 64 of 2000 31 / 65, 200 of 1000 76 / 87; at
+//   64, 4 of 4000 26.6 / 26.6, 64 of 8000 107 / 158 (8 query and key heads, e4m3, 64 of up to 500: 55 / 50); at 128,
+//   75 / 72, 57 / 70 and 183 / 167.  To 64 rows 32.  At 256 values a head the two are even sooner: at 48, 4 of 4000 45 / 37,
+//   64 of 2000 58 / 101, 24 of 4000 74 / 75; to 32 rows there.
+// * 128 rows or 256, which 8 wavefronts share, at 128: 72 / 70, 167 / 152 (64 values a head, 8 key heads: 24 of 4000
+//   100 / 105, 64 of 8000 469 / 409); 256 from 129 on, and never for more than 128 values, whose sums fill the registers.
+// A batch of prompts and single tokens takes what its mean asks for: a prompt of 2000 and 60 single tokens of
+// 1000-8000 125 (152 in tiles of 32), of 500 105 (57 in tiles of 32).
+//
+// Shares for a workgroup a CU, two of few rows with 64 values a head (kv_attn_split_kernel): one / two at 16 rows, 24
+// sequences in a window of 2000 26 / 23, 64 of up to 8190 63 / 56, 4 of 40,000 36 / 37; at 32 rows 32 / 29, 83 / 68,
+// 50 / 48; alike with e4m3 and pages of 16.  None for batches that one workgroup cannot count, and none for
+// prompts of two row tiles a CU and more.  Cut / whole, 4 prompts: 256 row tiles 53 / 50, 384 117 / 68, 512 144 / 99,
+// 1024 503 / 333; behind 4000 tokens each 128 115 / 144, 256 193 / 172, 320 246 / 288, 384 301 / 308, 448 363 / 328.
+// What lies behind a prompt only the device knows; whole tiles never lose from 448 on.
 static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
                           int64_t q_heads) {
   const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch, cus = device_cu_count();
   AttnPlan P;
-  P.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 || D > 128 ? 128 : 256;
+  P.rows = rows <= 16 ? 16 : rows <= (D <= 192 ? 64 : 32) ? 32 : rows <= 128 || D > 128 ? 128 : 256;
   const int64_t row_tiles = tokens * group / P.rows + batch + 1;
   P.shares = ((P.rows <= 32 && D == 64 ? 2 : 1) * cus + heads - 1) / heads;
   const int64_t most = row_tiles * ((width * block + 255) / 256 + 1);       // of 4 tiles each

@@ -320,10 +320,10 @@ def test_many_row_tiles(B, n):
                                          (1, 4, 192, 32, {"causal": False}), (2, 2, 128, 128, {}),
                                          (1, 3, 64, 16, {"window": 70})])
 def test_row_tiles_of_four_wavefronts(H, G, D, bs, kw, codes, value):
-    """At 33-128 rows a sequence and head, and at 192 and 256 values a head whatever the rows, a workgroup is 4
+    """At 65-128 rows a sequence and head, and at 192 and 256 values a head for more too, a workgroup is 4
     wavefronts and its ring of keys has two slots: each wavefront has read the first tile of keys before any
     writes the third over it.  Prompts of one to eight tiles, several row tiles a workgroup."""
-    n = 20 if D <= 128 else 150
+    n = 50 if D <= 128 else 150
     lens, news = [n + 300, n, n + 30, 3 * n + 64, n + 1], [n, n, n - 3, n + 5, 1]
     check(H, G, D, bs, codes, value, lens, news, **kw)
 
