@@ -51,6 +51,18 @@ def test_single_tokens_of_wide_groups(G, D):
     check(1, G, D, 64, INT8, F16, [1, 64, 65, 200, 777], [1] * 5, cu=False)
 
 
+@pytest.mark.parametrize("codes", [INT8, E4M3])
+@pytest.mark.parametrize("value", [F16, BF16])
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("G,new,window", [(4, 2, 0), (8, 4, 50), (4, 28, 0), (4, 80, 70)])
+def test_every_kernel(G, new, window, D, bs, value, codes):
+    """Every compiled form of the two kernels, at 8, 32, 112 and 320 rows a sequence and head: ragged lengths, the longest of
+    several runs, one sequence without tokens and one as long as its tokens."""
+    lens, news = [new + 231, 7, new, new + 65], [new, 0, new, max(1, new - 3)]
+    check(2, G, D, bs, codes, value, lens, news, window=window, extra=1)
+
+
 @pytest.mark.parametrize("codes,value", [(INT8, F16), (E4M3, BF16)])
 @pytest.mark.parametrize("L", [1023, 1024, 4097, 20000])
 def test_one_long_sequence(L, codes, value):

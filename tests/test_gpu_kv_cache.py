@@ -48,6 +48,28 @@ def test_append_matches_the_definition(H, D, bs, dtype, value):
 
 
 @pytest.mark.parametrize("dtype", CODES)
+@pytest.mark.parametrize("value", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_every_kernel(D, bs, value, dtype):
+    """Every compiled form of append and read: a new page, the end of a page and the next, a whole page and a piece."""
+    lens, news = [3, bs + 2, 2 * bs, bs - 1], [3, 5, bs, 2]
+    parts, table, k, v = problem(2, D, bs, dtype, lens, news, D + bs, value)
+    want = append(parts, k, v, table, lens, news)
+    cache = call(parts, table, k, v, lens, news)
+    same(cache, want)
+    for out in (torch.float16, torch.bfloat16, torch.float32):
+        got = kv_read(cache, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), offsets(news).to(DEV),
+                      total=sum(news), dtype=out)
+        at = 0
+        for b, n in enumerate(news):
+            for h in range(2):
+                for x, full in zip(got, gather(want, table[b], lens[b], h)[:2]):
+                    assert torch.equal(x[at:at + n, h].cpu(), full[lens[b] - n:].float().to(out)), (b, h, out)
+            at += n
+
+
+@pytest.mark.parametrize("dtype", CODES)
 @pytest.mark.parametrize("grow", [1e-3, 1.0, 300.0])
 def test_single_tokens_where_the_scale_grows_or_not(dtype, grow):
     """One token a sequence at every kind of place in a page: the first, in the middle, the last."""
