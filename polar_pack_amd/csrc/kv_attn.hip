@@ -31,7 +31,8 @@ namespace pp {
 // (and 65 / 69 at the long sequences, whose join reads half as many parts); a turn counted as 16 tiles
 // against 4 66.4 -> 63.2.  With 64 values a head a workgroup's registers leave room for a second on the CU, and
 // a tile is half the bytes on its way: 24 sequences of 5 drafted tokens in a window of 2000, 34.5 -> 30.7 us with
-// two.  V with the streaming cache policy, since a load takes whole lines of it; not K,
+// two.  64 sequences of 77-8190 with 4 key heads of 192: 80 us (5.2 TB/s); of 256 105 (5.3), where 48-76 bytes a lane
+// spill in tiles of 16 rows and 152-200 in tiles of 32.  V with the streaming cache policy, since a load takes whole lines of it; not K,
 // whose lines two loads share.
 template <int I>
 using Int = std::integral_constant<int, I>;

@@ -17,6 +17,9 @@
 // heads of 128: 102 us, 0.67 PFLOP/s of 1.35 that the library's fp16 product reaches; 509 tokens behind
 // 32,192: 166 us, 0.82.  Measured on the way (prompts / piece): wavefronts of 64 rows, one a SIMD 395 / 442 us (registers spilled),
 // 8 of 32 rows 142 / 182, a barrier apart 144 / 167, heavy row tiles first and priority 103 / 164.
+// 192 and 256 values a head: sums and queries of 32 rows take 144 and 192 registers, so 4 wavefronts, one a SIMD,
+// whose products wait for their weights; at 256 28 bytes a lane spill.  The same prompts with 12 query and 4 key heads of 192
+// 175 us, 0.44 PFLOP/s (a piece 272, 0.56), with 16 and 1 of 256 278, 0.50 (424, 0.64).
 #include "kv_attn.h"
 
 namespace pp {

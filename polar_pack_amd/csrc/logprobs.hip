@@ -12,7 +12,7 @@
 //
 // What bounds it: without alternatives the reading (2047 rows of 151,936 in float32, 1.24 GB: 219 us, 5.7
 // TB/s); with alternatives instructions and latency (250 rows in bf16 with 20 alternatives, 76 MB: 47 us; 22
-// instructions a logit, the vector units 45 % busy, two barriers a step).  A first floor from the threads'
+// instructions a logit, the vector units 56 % busy, two barriers a step).  A first floor from the threads'
 // largest logits and tests as floats before keys are made took it from 56 to 47; 4 workgroups a CU
 // instead of 2 cost 69 (each part picks its own list), 1 a CU 62.
 #include "kv_common.h"

@@ -40,7 +40,9 @@ class KVCache:
 
     ``k`` codes (pages, heads, block, D) and ``v`` codes (pages, heads, D, block), int8 or
     float8_e4m3fn; ``k_scale`` and ``v_scale`` float32 (pages, heads).  A value is code * scale.
-    Scales are 2**-64 or more (smaller ones count as that in an attention's values) or not finite;
+    Scales are 2**-64 or more (smaller ones count as that in an attention's values) or not finite, and
+    the value scales of the pages that one row sees are within a factor of 2**100 (past that its sum of
+    weights loses the pages of the smaller ones);
     codes of tokens before a sequence's length are finite, as :func:`kv_append` writes them: a NaN code put
     there by other means may reach rows that do not see it.  What lies past the lengths may hold anything.
     :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.

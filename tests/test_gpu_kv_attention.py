@@ -176,6 +176,17 @@ def test_scales_far_apart(many):
 
 
 @pytest.mark.parametrize("many", [1, 150])
+@pytest.mark.parametrize("large", [0, 1])
+def test_value_scales_as_far_apart_as_they_may_be(large, many):
+    """The pages of the smaller scale add nothing to the values but count in the sum of weights."""
+    def edit(parts, table, q):
+        of = table[0].long()
+        parts[3][of[large::2]] = 2.0 ** 40
+        parts[3][of[1 - large::2]] = 2.0 ** -60
+    check(1, 8, 128, 64, INT8, BF16, [900], [many], edit=edit)
+
+
+@pytest.mark.parametrize("many", [1, 150])
 @pytest.mark.parametrize("value,q_scale", [(F16, 1e-6), (F16, 2000.0), (BF16, 1e-30), (BF16, 1e6)])
 def test_queries_of_any_size(value, q_scale, many):
     """Subnormal and huge queries; with huge ones a row is one key's value."""
