@@ -741,14 +741,20 @@ int pp_dual_plug_table(const void* codes, int64_t n_codes, int code_layout, cons
 /* attention, log probabilities.  They have no counterpart in the reference.  */
 /* ------------------------------------------------------------------------ */
 
-/* Codes of a cache: int8 in -127..127, or float8 e4m3 (finite, no infinities). */
-enum pp_kv_codes { PP_KV_INT8 = 0, PP_KV_E4M3 = 1 };
+/* Codes of a cache: int8 in -127..127, float8 e4m3 (finite, no infinities), or 4-bit e2m1. */
+enum pp_kv_codes { PP_KV_INT8 = 0, PP_KV_E4M3 = 1, PP_KV_E2M1 = 2 };
 
 /*
  * A paged cache: `pages` pages of `block` tokens (16, 32, 64 or 128) for `heads` heads of
  * head_dim (64, 128, 192 or 256) values.  One byte a value: k is [page][head][token][d],
  * v is [page][head][d][token], both dense at a 16-byte boundary; k_scale and v_scale are
- * [page][head].  A value is code * scale.
+ * [page][head] float32.  A value is code * scale.
+ *
+ * In 4 bits (PP_KV_E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 for codes 0..7, bit 3 the sign) a byte holds two codes, the
+ * earlier one in its low half: k is [page][head][token][d / 2], v [page][head][d][token / 2].  Every 32 values
+ * d of a token and head share a scale, a power of two from 2^-14 to 2^13 held as a float8 e5m2 byte:
+ * k_scale is [page][head][token][d / 32], v_scale [page][head][d / 32][token], at 16-byte boundaries.  A k_scale of
+ * NaN marks a token whose keys or values were not finite.
  *
  * The sequences of a call: token t of sequence b lies in page table[b*table_ld + t / block]
  * at place t % block; the call's tokens cu[b] .. cu[b+1]-1 (cu[0] taken as 0) are the last ones of
@@ -760,8 +766,8 @@ enum pp_kv_codes { PP_KV_INT8 = 0, PP_KV_E4M3 = 1 };
 typedef struct pp_kv_cache {
   void* k;
   void* v;
-  float* k_scale;
-  float* v_scale;
+  void* k_scale;
+  void* v_scale;
   int64_t pages;
   int32_t heads, head_dim, block, codes;
 } pp_kv_cache;
@@ -777,6 +783,11 @@ typedef struct pp_kv_cache {
  * A value that is not finite makes the page's scale not finite (and its codes 0), so that every row
  * that sees the page is NaN, until the page begins anew.  A page that gets tokens belongs to one
  * sequence of the call.
+ *
+ * In 4 bits a token's codes are its own: scale is the smallest power of two from 2^-14 to 2^13 with
+ * max|x| <= 7 * scale over the group's 32 values, and code the nearest to x / scale, ties to even, held to
+ * +-6.  Both are exact functions of x.  A token and head with a key or a value that is not finite gets NaN in all its
+ * k_scales: every row that sees the token is NaN, and it reads NaN.
  */
 int pp_kv_append(const pp_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
                  int64_t v_sh, int dtype, int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
@@ -823,6 +834,46 @@ int64_t pp_logprobs_workspace_size(int64_t rows, int64_t V, int64_t top);
 int pp_logprobs(const void* logits, int64_t l_st, int dtype, int64_t rows, int64_t V, const int64_t* tokens,
                 int64_t t_st, int64_t per_row, int64_t top, float* logprob, float* entropy, int64_t* top_ids,
                 float* top_logprobs, void* workspace, int64_t workspace_size, void* stream);
+
+/*
+ * Rotary positions.  Of a row's values the first rotary_dim (a multiple of 16) are turned in pairs, f with
+ * f + rotary_dim / 2 (PP_PAIRS_HALVES) or 2f with 2f + 1 (PP_PAIRS_NEIGHBOURS):
+ *   a' = scaling * (a cos w - b sin w),  b' = scaling * (b cos w + a sin w),
+ *   w = 2 pi * position * turns[f] / 2^64,
+ * position that of the row's token on axis axes[f]; the rest is copied.  turns (device) is each pair's
+ * frequency, the fraction of a turn that one step is, times 2^64; with it the angle is exact for every 64-bit
+ * position, negative ones (which turn back) among them.  axes (device; null: all 0) holds numbers below n_axes.
+ */
+enum pp_pairs { PP_PAIRS_HALVES = 0, PP_PAIRS_NEIGHBOURS = 1 };
+enum pp_positions { PP_POS_I32 = 0, PP_POS_I64 = 1 };
+typedef struct pp_rotary {
+  const uint64_t* turns;
+  const uint8_t* axes;
+  int32_t rotary_dim, n_axes, pairs;
+  float scaling;
+} pp_rotary;
+
+/*
+ * Rows (token, head) of head_dim values (a multiple of 8, at most 512; PP_F16, PP_BF16 or PP_F32) at
+ * x + token*x_st + head*x_sh, turned in float32 and rounded once, to out + token*o_st + head*o_sh; out may be x with
+ * x's strides, and otherwise does not overlap it.  The position of a token on axis a is positions[a*pos_ld + token].
+ */
+int pp_rotate(const void* x, int64_t x_st, int64_t x_sh, int dtype, int64_t tokens, int64_t heads, int64_t head_dim,
+              const pp_rotary* rotary, const void* positions, int64_t pos_ld, int pos_type, void* out, int64_t o_st,
+              int64_t o_sh, void* stream);
+
+/*
+ * pp_kv_append with the keys turned on the way, and the queries beside them: k and v as pp_kv_append takes them, the
+ * keys turned in float32 (4 bits: in float64, so that each code is the nearest one) and not rounded in between;
+ * q (tokens, q_heads, head_dim) with strides q_st, q_sh turned and rounded to q_out, dense at a 16-byte boundary
+ * (q_heads 0: none).  positions as pp_rotate takes them, or null: a token's own place in its sequence, on every axis;
+ * the queries of tokens of no sequence (past cu[batch]) are zero then.
+ */
+int pp_kv_rotate_append(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads,
+                        void* q_out, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                        int64_t v_sh, int dtype, int64_t tokens, const pp_rotary* rotary, const void* positions,
+                        int64_t pos_ld, int pos_type, const int32_t* table, int64_t table_ld, int64_t table_width,
+                        const int32_t* lengths, const int32_t* cu, int64_t batch, void* stream);
 
 #ifdef __cplusplus
 }

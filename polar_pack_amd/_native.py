@@ -16,7 +16,9 @@ from .build import LIB
 
 PP_OK, PP_EINVAL, PP_EHIP, PP_ENOSUPPORT = 0, 1, 2, 3
 PP_F16, PP_F32, PP_BF16 = 0, 1, 2
-PP_KV_INT8, PP_KV_E4M3 = 0, 1
+PP_KV_INT8, PP_KV_E4M3, PP_KV_E2M1 = 0, 1, 2
+PP_PAIRS_HALVES, PP_PAIRS_NEIGHBOURS = 0, 1
+PP_POS_I32, PP_POS_I64 = 0, 1
 PP_DUAL_I16_OFFSET, PP_DUAL_U16_BE = 0, 1
 PP_QUAD_NK, PP_QUAD_KN = 0, 1
 PP_GEMM_ROWS, PP_GEMM_KN, PP_GEMM_GENERIC = 1, 2, 3
@@ -52,6 +54,12 @@ class DualProj(C.Structure):
     """``pp_dual_proj`` (include/polar_pack.h)."""
     _fields_ = [("codes", vp), ("ldc", i64), ("pos0", i64), ("x", vp), ("x_sm", i64),
                 ("out", vp * 2), ("o_sm", i64), ("N", C.c_int32), ("K", C.c_int32)]
+
+
+class Rotary(C.Structure):
+    """``pp_rotary`` (include/polar_pack.h)."""
+    _fields_ = [("turns", vp), ("axes", vp), ("rotary_dim", C.c_int32), ("n_axes", C.c_int32), ("pairs", C.c_int32),
+                ("scaling", C.c_float)]
 
 
 class KVCache(C.Structure):
@@ -149,6 +157,9 @@ EXPORTS = {
                               vp, i64, vp, i64, vp]),
     "pp_logprobs_workspace_size": (i64, [i64, i64, i64]),
     "pp_logprobs": (i32, [vp, i64, i32, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp]),
+    "pp_rotate": (i32, [vp, i64, i64, i32, i64, i64, i64, vp, vp, i64, i32, vp, i64, i64, vp]),
+    "pp_kv_rotate_append": (i32, [vp, vp, i64, i64, i64, vp, vp, i64, i64, vp, i64, i64, i32, i64, vp, vp, i64, i32, vp,
+                                  i64, i64, vp, vp, i64, vp]),
     "pp_upload": (i32, [vp, vp, i64, vp]),
     "pp_upload_tables": (i32, [vp, vp, vp, i32, vp]),
 }

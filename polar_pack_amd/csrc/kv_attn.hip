@@ -471,6 +471,7 @@ extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t 
   if (rc) return rc;
   rc = kv_check_seqs(A.C, table, table_ld, table_width, lengths, cu, batch, tokens, &A.S);
   if (rc) return rc;
+  PP_REQUIRE(cache->codes != PP_KV_E2M1, "pp_kv_attention: not yet for 4-bit codes");
   PP_REQUIRE(dtype == PP_F16 || dtype == PP_BF16, "pp_kv_attention: dtype %d is not PP_F16 or PP_BF16", dtype);
   PP_REQUIRE(q_heads > 0 && q_heads % A.C.heads == 0 && q_heads <= 65535,
              "pp_kv_attention: %lld query heads over %d heads", (long long)q_heads, A.C.heads);

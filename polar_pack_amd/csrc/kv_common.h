@@ -1,4 +1,4 @@
-// The 8-bit key/value cache: its layout, the sequences of a call and the codes.
+// The key/value cache in 8 or 4 bits: its layout, the sequences of a call and the codes.
 //
 // A cache is `pages` pages of `block` tokens (16, 32, 64 or 128) for `heads` heads of D values:
 //   K codes [page][head][token][D], V codes [page][head][D][token], one byte a value, and one
@@ -6,6 +6,13 @@
 // V is kept transposed because a matrix-core operand of the product with the weights wants
 // consecutive tokens of one d in a lane: here those are 16 consecutive bytes, and no kernel
 // transposes V through LDS.
+//
+// In 4 bits (PP_KV_E2M1) a byte holds two codes, of neighbouring d (K) or tokens (V), and every 32 values d of a
+// token and head have a scale of their own, a power of two as an e5m2 byte: K [page][head][token][D / 32],
+// V [page][head][D / 32][token].  Powers of two make the codes exact functions of the values, whatever the order of
+// operations, let the conversion to halves take K's scale along, and leave code * scale exact in fp16; as the upper
+// byte of an fp16 number a V scale becomes a factor by one permute.  A token's codes depend on no other token, so an
+// append never rounds again what is there.
 #pragma once
 
 #include "pp_common.h"
@@ -24,11 +31,13 @@ constexpr float KV_SCALE_MIN = 5.421010862427522e-20f;   // 2^-64
 struct KvCache {
   uint8_t* k;
   uint8_t* v;
-  float* ks;
+  float* ks;        // in 4 bits bytes: scales_k, scales_v
   float* vs;
   int64_t pages;
   int heads, block, shift;   // block == 1 << shift
 };
+__device__ __forceinline__ uint8_t* scales_k(const KvCache& C) { return reinterpret_cast<uint8_t*>(C.ks); }
+__device__ __forceinline__ uint8_t* scales_v(const KvCache& C) { return reinterpret_cast<uint8_t*>(C.vs); }
 
 // The sequences of a call: token t of sequence b lies in page table[b*ld + t / block].  The call's
 // tokens cu[b] .. cu[b+1]-1 are the last of sequence b's lengths[b] tokens; without cu every
@@ -130,6 +139,16 @@ struct KvCodes<PP_KV_E4M3> {
     x[0] = lo[0]; x[1] = lo[1]; x[2] = hi[0]; x[3] = hi[1];
   }
 };
+
+// Scales of 4-bit codes: the exponent of the smallest power of two from 2^-14 to 2^13 that is a seventh of the
+// magnitude `bits` or more, its float and its byte.
+__device__ __forceinline__ int scale4(uint32_t bits) {
+  const int e = (int)((bits + 0x1fffffu) >> 23) - 129;      // past 1.75 * 2^k: one more
+  return min(max(e, -14), 13);
+}
+__device__ __forceinline__ float scale4_value(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t scale4_byte(int e) { return (uint32_t)(e + 15) << 2; }
+constexpr uint32_t SCALE4_NAN = 0x7f;
 
 // 16-bit values in memory as float and back.
 struct IoF16 {

@@ -1,0 +1,106 @@
+// Queries and keys turned by their positions, keys and values written to the cache, in one launch: 8 bits and the
+// entry point.
+#include "kv_cache4.h"
+#include "rotate_keys.h"
+
+namespace pp {
+
+struct RotateArgs {
+  AppendArgs A;
+  Rot R;
+  RotRows Q;
+  int per, chunks, table;    // heads a workgroup, workgroups a page and side, whether there is a table
+  unsigned units;            // workgroups that append; the others turn queries
+};
+
+template <int CODES, typename IO, int D>
+__global__ __launch_bounds__(4 * D) void kv_rotate_append_kernel(const RotateArgs X) {
+  if (blockIdx.x >= X.units) {
+    rotate_queries<IO>(X.A.S, X.R, X.Q, blockIdx.x - X.units);
+    return;
+  }
+  const AppendArgs& A = X.A;
+  const KvCache& C = A.C;
+  const uint32_t n = 2 * (uint32_t)X.chunks, item = blockIdx.x / n, r = blockIdx.x - item * n;
+  const int isv = r >= (uint32_t)X.chunks, h0 = (int)(isv ? r - X.chunks : r) * X.per, h1 = min(h0 + X.per, C.heads);
+  Piece P;
+  if (!kv_piece(C, A.S, (int)item, C.shift, P) || P.page < 0) return;
+  __shared__ uint32_t red[16];
+  extern __shared__ __align__(16) uint32_t lds[];      // of keys the table, of values the codes
+  const bool mine = (int)threadIdx.x < (C.block / 4) * (D / 8);
+  Trig<float>* const tab = X.table ? reinterpret_cast<Trig<float>*>(lds) : nullptr;
+  if (!isv && tab) {
+    rot_table(X.R, P, tab);
+    __syncthreads();
+  }
+  for (int head = h0; head < h1; ++head) {
+    const uint16_t* src = A.x[isv] + (int64_t)head * A.sh[isv];
+    if (isv) {
+      u32x4 x[4];
+      const uint32_t top = load_unit<D>(P, src, A.st[1], A.vec, mine, x);
+      append_page<CODES, D>(C, P, head, 1, top, [](uint32_t w) { return mag(IO::get((uint16_t)w)); }, red, lds,
+                            [&](int i, int j) { return half_of<IO>(x[i], j); });
+    } else {
+      float x[4][8];
+      load_turned<IO, float, D>(X.R, P, src, A.st[0], A.vec, mine, tab, x);
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, mag(x[i][j]));
+      append_page<CODES, D>(C, P, head, 0, top, [](uint32_t w) { return w; }, red, lds,
+                            [&](int i, int j) { return x[i][j]; });
+    }
+    if (head + 1 < h1) __syncthreads();                // LDS is read
+  }
+}
+
+}  // namespace pp
+
+using namespace pp;
+
+extern "C" int pp_kv_rotate_append(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads,
+                                   void* q_out, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                                   int64_t v_sh, int dtype, int64_t tokens, const pp_rotary* rotary,
+                                   const void* positions, int64_t pos_ld, int pos_type, const int32_t* table,
+                                   int64_t table_ld, int64_t table_width, const int32_t* lengths, const int32_t* cu,
+                                   int64_t batch, void* stream) {
+  RotateArgs X;
+  int rc = append_check("pp_kv_rotate_append", cache, k, k_st, k_sh, v, v_st, v_sh, dtype, tokens, table, table_ld,
+                        table_width, lengths, cu, batch, &X.A);
+  if (rc) return rc;
+  const int D = cache->head_dim;
+  rc = rot_check(rotary, positions, pos_ld, pos_type, tokens, D, false, &X.R);
+  if (rc || tokens == 0) return rc;
+  PP_REQUIRE(q_heads >= 0 && q_heads <= 65535, "pp_kv_rotate_append: %lld query heads", (long long)q_heads);
+  X.Q = RotRows{q_heads ? q : nullptr, q_out, q_st, q_sh, q_heads * D, D, (int)tokens, (int)q_heads, D, 1, 0};
+  if (X.Q.x) {
+    PP_REQUIRE(q_out && aligned(q, 2) && aligned(q_out, 16), "pp_kv_rotate_append: queries or their output null or not aligned");
+    X.Q.vec = aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0;
+    const int64_t groups = rot_groups(tokens * rot_units(X.R.half, D), q_heads);
+    X.Q.per = (int)((q_heads + groups - 1) / groups);
+  }
+  PP_REQUIRE(X.Q.x || q_heads == 0, "pp_kv_rotate_append: null queries");
+  if (cache->codes == PP_KV_E2M1) return kv_append4(X.A, &X.R, &X.Q, D, dtype, (hipStream_t)stream);
+  const KvCache& C = X.A.C;
+  const int64_t items = kv_pieces(X.A.S, C.shift);
+  const dim3 wg(unit_threads(C.block, D));
+  X.per = heads_per(2 * items, C.heads);
+  X.chunks = (C.heads + X.per - 1) / X.per;
+  const int64_t units = items * 2 * X.chunks, blocks = units + query_blocks(X.R, X.Q, wg.x);
+  PP_REQUIRE(blocks <= UINT32_MAX / wg.x, "pp_kv_rotate_append: too many tokens and sequences");
+  X.units = (unsigned)units;
+  // a piece of a call without cu is one token
+  const int64_t table_bytes = (cu ? C.block : 1) * (int64_t)X.R.half * (int64_t)sizeof(Trig<float>);
+  X.table = table_bytes <= ROT_TABLE_MAX;
+  const unsigned tile = tile_bytes(C.block, D), lds = X.table && table_bytes > tile ? (unsigned)table_bytes : tile;
+  return by_width(D, [&](auto d) -> int {
+    constexpr int W = decltype(d)::value;
+    const bool i8 = cache->codes == PP_KV_INT8, h = dtype == PP_F16;
+    auto kern = i8 ? (h ? kv_rotate_append_kernel<PP_KV_INT8, IoF16, W> : kv_rotate_append_kernel<PP_KV_INT8, IoBf16, W>)
+                   : (h ? kv_rotate_append_kernel<PP_KV_E4M3, IoF16, W> : kv_rotate_append_kernel<PP_KV_E4M3, IoBf16, W>);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), wg, lds, (hipStream_t)stream, X);
+    PP_LAUNCH_CHECK();
+    return PP_OK;
+  });
+}

@@ -1,15 +1,18 @@
-"""An 8-bit key/value cache and the attention that reads it.
+"""A key/value cache in 8 or 4 bits and the attention that reads it.
 
-The cache is paged: a page holds ``block`` tokens of every head, one byte a value, with one float32
-scale for each page and head of the keys and of the values.  A sequence is a row of a block table;
-the packed models of a stream are rows of one table, so that one launch serves all of them.
+The cache is paged: a page holds ``block`` tokens of every head, one byte a value with one float32
+scale for each page and head of the keys and of the values, or half a byte a value with a scale for every 32
+values of a token.  A sequence is a row of a block table; the packed models of a stream are rows of one table, so
+that one launch serves all of them.
 
-* :class:`KVCache`       -- the pages
-* :func:`kv_append`      -- new keys and values of a step or a prompt
-* :func:`kv_attention`   -- attention of the new tokens to everything before and among them
-* :func:`kv_read`        -- tokens of the cache as plain values
+* :class:`KVCache`            -- the pages in 8 bits
+* :class:`KVCache4`           -- the pages in 4 bits
+* :func:`kv_append`           -- new keys and values of a step or a prompt
+* :func:`kv_rotate_append`    -- the same with the keys, and the queries, turned by their positions first
+* :func:`kv_attention`        -- attention of the new tokens to everything before and among them
+* :func:`kv_read`             -- tokens of the cache as plain values
 
-All three take the same description of a call: ``block_table`` (B, width) int32, ``lengths`` (B,)
+All take either cache and the same description of a call: ``block_table`` (B, width) int32, ``lengths`` (B,)
 int32 (the tokens of each sequence *after* the call's own) and ``cu`` (B + 1,) int32, the offsets of
 each sequence's tokens among the call's (None: one token each).  They stay on the device; nothing
 here waits for it, and every call can be captured in a HIP graph.  What the three tensors hold is
@@ -27,6 +30,7 @@ import math
 import torch
 
 from . import _native as nat
+from .rotary import _check_rotary, _positions
 
 BLOCKS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 192, 256)
@@ -81,9 +85,56 @@ class KVCache:
         return cls(k.view(dtype), v.view(dtype), k_scale, v_scale)
 
 
+class KVCache4:
+    """The pages of a cache in 4 bits.
+
+    A value is code * scale.  Codes are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 for 0..7, bit 3 the sign), two a byte, the
+    earlier one in its low half: ``k`` uint8 (pages, heads, block, D / 2), ``v`` uint8 (pages, heads, D, block / 2).
+    Every 32 values of a token and head share a scale, a power of two from 2**-14 to 2**13 as float8_e5m2:
+    ``k_scale`` (pages, heads, block, D / 32), ``v_scale`` (pages, heads, D / 32, block).  4.25 bits a value; a
+    token's codes depend on no other token.  A NaN in a token's ``k_scale`` makes the token NaN for every row that
+    sees it; scales of tokens before a sequence's length are otherwise as :func:`kv_append` writes them.  What lies past
+    the lengths may hold anything.
+    :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.
+    """
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dim() != 4 or k.dtype != torch.uint8:
+            raise TypeError("k must be uint8 (pages, heads, block, D / 2)")
+        pages, heads, block, D = k.shape
+        D *= 2
+        if block not in BLOCKS or D not in HEAD_DIMS:
+            raise ValueError(f"block must be one of {BLOCKS} and D one of {HEAD_DIMS}, got {block} and {D}")
+        if v.dtype != torch.uint8 or v.shape != (pages, heads, D, block // 2):
+            raise ValueError("v must be uint8 (pages, heads, D, block / 2)")
+        for s, shape in ((k_scale, (pages, heads, block, D // 32)), (v_scale, (pages, heads, D // 32, block))):
+            if s.dtype != torch.float8_e5m2 or s.shape != shape:
+                raise ValueError(f"k_scale and v_scale must be float8_e5m2 (pages, heads, block, D / 32) and "
+                                 f"(pages, heads, D / 32, block)")
+        ts = (k, v, k_scale, v_scale)
+        if k.device.type != "cuda" or any(t.device != k.device for t in ts):
+            raise ValueError("a cache's tensors must be on one ROCm device")
+        if not all(t.is_contiguous() and not t.is_neg() for t in ts):
+            raise ValueError("a cache's tensors must be contiguous and hold their values as they are")
+        if pages < 1 or heads < 1 or any(t.data_ptr() % 16 for t in ts):
+            raise ValueError("a cache needs a page and a head, and codes and scales at 16-byte boundaries")
+        self.k, self.v, self.k_scale, self.v_scale = ts
+        self.pages, self.heads, self.block, self.head_dim = pages, heads, block, D
+        self.device = k.device
+        self._abi = nat.KVCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, D,
+                                block, nat.PP_KV_E2M1)
+        self._ref = ctypes.addressof(self._abi)
+
+    @classmethod
+    def zeros(cls, pages, heads, head_dim, *, block=64, device="cuda"):
+        shapes = ((block, head_dim // 2), (head_dim, block // 2), (block, head_dim // 32), (head_dim // 32, block))
+        k, v, k_scale, v_scale = (torch.zeros((pages, heads) + s, dtype=torch.uint8, device=device) for s in shapes)
+        return cls(k, v, k_scale.view(torch.float8_e5m2), v_scale.view(torch.float8_e5m2))
+
+
 def _check_cache(cache):
-    if not isinstance(cache, KVCache):
-        raise TypeError("cache must be a KVCache")
+    if not isinstance(cache, (KVCache, KVCache4)):
+        raise TypeError("cache must be a KVCache or a KVCache4")
 
 
 def _call(cache, block_table, lengths, cu, tokens):
@@ -135,6 +186,14 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
     ``round(code * (old / scale))``.  A value that is not finite makes its page's scale
     not finite, so that every row that sees the page is NaN.  A page that gets tokens must belong
     to one sequence of the call (shared pages are for tokens already written).
+
+    In 4 bits, for every 32 values of a token and head::
+
+        scale = the smallest power of two in [2**-14, 2**13] with max|x| <= 7 * scale
+        code  = the nearest to x / scale           ties to even, held to +-6
+
+    Both are exact functions of the values.  A value that is not finite, of the key or the value, makes the
+    token NaN for every row that sees it, and where it is read.
     """
     _check_cache(cache)
     k = _values(cache, k, "k", cache.heads)
@@ -147,6 +206,43 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
         nat.check(nat.lib().pp_kv_append(cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                                          v.stride(0), v.stride(1), _VALUES[k.dtype], n, *call,
                                          nat.raw_stream(cache.device)), "pp_kv_append")
+
+
+def kv_rotate_append(cache, q, k, v, rotary, block_table, lengths, cu=None, *, positions=None):
+    """:func:`kv_append` with the keys turned by ``rotary`` (a :class:`polar_pack_amd.rotary.Rotary`) on the way;
+    returns the queries ``q`` (tokens, q_heads, D) turned, in their type, in the same launch.  ``q`` may be None,
+    then None is returned.
+
+    ``positions``: (tokens,), or (axes, tokens), int32 or int64, as :func:`polar_pack_amd.rotary.rotate` takes them;
+    None: each token's own place in its sequence, ``lengths[b] - n_b + i``, on every axis, and queries of tokens of no
+    sequence (past ``cu[B]``) are zero.  Turned keys are not rounded before their codes are: they are float32, for a
+    cache of 4 bits float64.
+    """
+    _check_cache(cache)
+    dev, D = cache.device, cache.head_dim
+    k = _values(cache, k, "k", cache.heads)
+    v = _values(cache, v, "v", cache.heads)
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must have one shape and type")
+    n = k.shape[0]
+    if q is not None:
+        q = _values(cache, q, "q", None)
+        if q.shape[0] != n or q.dtype != k.dtype:
+            raise ValueError("q must have k's tokens and type")
+    _check_rotary(rotary, D, dev)
+    at = (None, 0, nat.PP_POS_I32)
+    if positions is not None:
+        positions, at = _positions(rotary, positions, n, dev)
+    call = _call(cache, block_table, lengths, cu, n)
+    with nat.on_device(dev):
+        queries, out = (None, 0, 0, 0, None), None
+        if q is not None:
+            out = torch.empty((n, q.shape[1], D), dtype=q.dtype, device=dev)
+            queries = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], out.data_ptr())
+        nat.check(nat.lib().pp_kv_rotate_append(cache._ref, *queries, k.data_ptr(), k.stride(0), k.stride(1),
+                                                v.data_ptr(), v.stride(0), v.stride(1), _VALUES[k.dtype], n,
+                                                rotary._ref, *at, *call, nat.raw_stream(dev)), "pp_kv_rotate_append")
+    return out
 
 
 def kv_read(cache, block_table, lengths, cu=None, *, total=None, dtype=torch.float16):
