@@ -875,6 +875,24 @@ int pp_kv_rotate_append(const pp_kv_cache* cache, const void* q, int64_t q_st, i
                         int64_t pos_ld, int pos_type, const int32_t* table, int64_t table_ld, int64_t table_width,
                         const int32_t* lengths, const int32_t* cu, int64_t batch, void* stream);
 
+/*
+ * Drafted tokens against the target's probabilities.  Sequence b has counts[b] drafts (held to 0..n; counts null: n)
+ * tokens[b*t_sb + i], the target's rows target + b*p_sb + i*p_sr for i = 0..n and the draft's rows draft + b*q_sb +
+ * i*q_sr for i < n, of V probabilities (PP_F16, PP_BF16 or PP_F32; draft null: the drafts were certain), and numbers
+ * uniforms[b*u_sb + i] in [0, 1), i = 0..n.  accepted[b] is the number of first drafts with
+ *   u_i q_i(token) < p_i(token),
+ * and out[b*(n+1) ..] these tokens, then one drawn with u_n, then -1.  It is drawn from max(p_i - q_i, 0) at a draft
+ * that was refused (from p_i where that is nothing; without draft from p_i but the refused token), from p_count after
+ * the last: the first t whose sum of entries 0..t passes u_n times the sum of all, in float64.  An entry that is not
+ * a positive finite number counts as 0, so does a token outside [0, V); a row of nothing else gives -1.  The workspace
+ * (pp_verify_drafts_workspace_size bytes) needs no initial values; done (4 * batch bytes) is zero on entry and left zero.
+ */
+int64_t pp_verify_drafts_workspace_size(int64_t batch, int64_t V);
+int pp_verify_drafts(const void* target, int64_t p_sb, int64_t p_sr, const void* draft, int64_t q_sb, int64_t q_sr,
+                     int dtype, int64_t batch, int64_t n, int64_t V, const int64_t* tokens, int64_t t_sb,
+                     const float* uniforms, int64_t u_sb, const int32_t* counts, int64_t* out, int64_t* accepted,
+                     void* workspace, int64_t workspace_size, void* done, int64_t done_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

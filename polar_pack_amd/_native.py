@@ -160,6 +160,9 @@ EXPORTS = {
     "pp_rotate": (i32, [vp, i64, i64, i32, i64, i64, i64, vp, vp, i64, i32, vp, i64, i64, vp]),
     "pp_kv_rotate_append": (i32, [vp, vp, i64, i64, i64, vp, vp, i64, i64, vp, i64, i64, i32, i64, vp, vp, i64, i32, vp,
                                   i64, i64, vp, vp, i64, vp]),
+    "pp_verify_drafts_workspace_size": (i64, [i64, i64]),
+    "pp_verify_drafts": (i32, [vp, i64, i64, vp, i64, i64, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp,
+                               i64, vp]),
     "pp_upload": (i32, [vp, vp, i64, vp]),
     "pp_upload_tables": (i32, [vp, vp, vp, i32, vp]),
 }
