@@ -22,7 +22,8 @@ SOURCES = ["capi.hip", "quad.hip", "quad_rows.hip", "quad_mfma.hip", "quad_big.h
            "quad_tile.hip", "quad_kn.hip", "dual.hip", "dual_rows.hip", "dual_strip.hip", "dual_tile.hip",
            "dual_kn.hip", "dual_mfma.hip", "pack.hip", "noalloc.hip", "kv_cache.hip",
            "kv_attn.hip", "kv_attn_many.hip", "logprobs.hip", "rotary.hip",
-           "kv_cache4.hip", "kv_rotate.hip", "drafts.hip"]
+           "kv_cache4.hip", "kv_rotate.hip", "drafts.hip",
+           "kv_attn4.hip", "kv_attn4_many.hip"]
 ARCH = "gfx950"
 
 # Packed FP32 instructions are disabled for all device code (their results have been

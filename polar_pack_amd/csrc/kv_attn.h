@@ -1,4 +1,4 @@
-// What the attention kernels of the 8-bit cache share: rows, what they see, runs of keys, queries.
+// What the attention kernels share: rows, what they see, runs of keys, queries.
 #pragma once
 
 #include "kv_common.h"
@@ -288,6 +288,26 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+// 8 codes of 4 bits as an operand of 8 halves, times `scale`, a power of two.
+__device__ __forceinline__ f16x8 halves4(uint32_t w, float scale) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The scales of 8 tokens as halves: a byte is the upper one of an fp16 number.
+__device__ __forceinline__ f16x8 scales4(uint32_t lo, uint32_t hi) {
+  const u32x4 w = {__builtin_amdgcn_perm(0u, lo, 0x010c000cu), __builtin_amdgcn_perm(0u, lo, 0x030c020cu),
+                   __builtin_amdgcn_perm(0u, hi, 0x010c000cu), __builtin_amdgcn_perm(0u, hi, 0x030c020cu)};
+  return __builtin_bit_cast(f16x8, w);
+}
+// Scales of tokens 4 w .. 4 w + 3 of which only the first `seen - 4 w` count.
+__device__ __forceinline__ uint32_t keep_bytes(int left) {
+  return left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+}
+
 // 16 codes as two operands of 8 halves.
 template <int CODES>
 __device__ __forceinline__ void to_halves(u32x4 w, f16x8& a, f16x8& b) {
@@ -303,29 +323,27 @@ __device__ __forceinline__ void to_halves(u32x4 w, f16x8& a, f16x8& b) {
   }
 }
 
-// A row's query as the second operand of S^T = K Q^T: lane group g holds values 64 j + 16 g + 8 e + 0..7
-// as q[j][e], scaled by a power of two so that the largest lies in [2^13, 2^14): bf16 queries of any
+// A row's query as the second operand of S^T = K Q^T: lane group g holds values EL g .. EL g + EL - 1 of every 4 EL
+// (EL 16, or 32 where a lane loads 32 codes of 4 bits), 8 after 8, scaled by a power of two so that the largest lies in [2^13, 2^14): bf16 queries of any
 // size fit in fp16 then.  With fp16's smallest step 2^-24 a bf16 value keeps all its bits down to 2^-30 of
 // the row's largest (an fp16 one to 2^-27); smaller ones lose some, and what is below 2^-38 of it is zero.
 // load_q issues the loads, make_q returns the factor of the row's sums, score scale and power of two; NaN for a
 // row that is not finite.
-template <int D>
-__device__ __forceinline__ void load_q(const AttnArgs& A, int token, int hq, int g, bool real, u32x4 (*w)[2]) {
-  const uint16_t* p = A.q + (int64_t)token * A.q_st + (int64_t)hq * A.q_sh + 16 * g;
+template <int D, int EL>
+__device__ __forceinline__ void load_q(const AttnArgs& A, int token, int hq, int g, bool real, u32x4* w) {
+  const uint16_t* p = A.q + (int64_t)token * A.q_st + (int64_t)hq * A.q_sh + EL * g;
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j)
+  for (int n = 0; n < D / 32; ++n) {
+    w[n] = u32x4{0, 0, 0, 0};
+    if (!real) continue;
+    const uint16_t* x = p + 4 * EL * (n / (EL / 8)) + 8 * (n % (EL / 8));
+    if (A.q_vec) {
+      w[n] = *reinterpret_cast<const u32x4*>(x);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[j][e] = u32x4{0, 0, 0, 0};
-      if (!real) continue;
-      const uint16_t* x = p + 64 * j + 8 * e;
-      if (A.q_vec) {
-        w[j][e] = *reinterpret_cast<const u32x4*>(x);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[j][e][k] = (uint32_t)x[2 * k] | (uint32_t)x[2 * k + 1] << 16;
-      }
+      for (int k = 0; k < 4; ++k) w[n][k] = (uint32_t)x[2 * k] | (uint32_t)x[2 * k + 1] << 16;
     }
+  }
 }
 
 // PARTS 16-byte pieces of a row as halves; the row's other pieces are in the lanes lane ^ FROM, lane ^ 2 FROM .. .
@@ -348,8 +366,8 @@ __device__ __forceinline__ float scale_q(const AttnArgs& A, const u32x4* w, f16x
 }
 
 template <typename IO, int D>
-__device__ __forceinline__ float make_q(const AttnArgs& A, const u32x4 (*w)[2], f16x8 (*q)[2]) {
-  return scale_q<IO, D / 32, 16>(A, &w[0][0], &q[0][0]);
+__device__ __forceinline__ float make_q(const AttnArgs& A, const u32x4* w, f16x8* q) {
+  return scale_q<IO, D / 32, 16>(A, w, q);
 }
 
 // The same for 32 rows a product: lane half hh holds values 16 c + 8 hh + 0..7 as q[c].
@@ -402,7 +420,9 @@ struct AttnPlan {
   int64_t shares, grid, bytes, counts;
 };
 
-// Prompts (kv_attn_many.hip).
+// Prompts (kv_attn_many.hip), and the 4-bit forms (kv_attn4.hip, kv_attn4_many.hip).
 int kv_attn_many(const AttnArgs& A, const AttnPlan& P, int D, int codes, int dtype, hipStream_t st);
+int kv_attn_split4(const AttnArgs& A, const AttnPlan& P, int D, int dtype, hipStream_t st);
+int kv_attn_many4(const AttnArgs& A, const AttnPlan& P, int D, int dtype, hipStream_t st);
 
 }  // namespace pp
