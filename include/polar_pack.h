@@ -883,8 +883,9 @@ int pp_kv_rotate_append(const pp_kv_cache* cache, const void* q, int64_t q_st, i
  *   u_i q_i(token) < p_i(token),
  * and out[b*(n+1) ..] these tokens, then one drawn with u_n, then -1.  It is drawn from max(p_i - q_i, 0) at a draft
  * that was refused (from p_i where that is nothing; without draft from p_i but the refused token), from p_count after
- * the last: the first t whose sum of entries 0..t passes u_n times the sum of all, in float64.  An entry that is not
- * a positive finite number counts as 0, so does a token outside [0, V); a row of nothing else gives -1.  The workspace
+ * the last: the first t whose sum of entries 0..t passes u_n times the sum of all, in float64.  A NaN
+ * or an entry below 0 counts as 0, infinity as the largest float32, a token outside [0, V) as one of probability 0; a
+ * row of nothing gives -1.  The workspace
  * (pp_verify_drafts_workspace_size bytes) needs no initial values; done (4 * batch bytes) is zero on entry and left zero.
  */
 int64_t pp_verify_drafts_workspace_size(int64_t batch, int64_t V);

@@ -8,16 +8,17 @@
 // smallest probabilities, and neighbouring tokens would change places.
 //
 // Only the row that is drawn from is read, cut into parts over workgroups.  Each finds the row by itself (two round
-// trips: tokens, then their probabilities), sums its part, and counts itself done; the one that counts last finds the
-// part in which the sum passes, reads that again and finds the token.  One launch, and the order of the sums is
-// fixed by the parts.
+// trips: tokens, then their probabilities), leaves the sum of every 1024 entries in the workspace, and counts itself
+// done; of the one that counts last a wavefront finds the 1024 in which the sum passes, reads those again and finds
+// the token.  One launch, and the order of the sums is fixed.
 #include "kv_common.h"
 
 namespace pp {
 
 constexpr int DR_THREADS = 256;
-constexpr int DR_PER = 16;                          // entries a thread and step
-constexpr int DR_STEP = DR_THREADS * DR_PER;
+constexpr int DR_PER = 16;                          // entries a lane and chunk
+constexpr int DR_CHUNK = 64 * DR_PER;
+constexpr int DR_STEP = DR_THREADS * DR_PER;        // a chunk for each wavefront
 
 struct DraftArgs {
   const void* p;
@@ -27,62 +28,73 @@ struct DraftArgs {
   const int32_t* counts;  // null: n of every sequence
   int64_t* out;
   int64_t* accepted;
-  double* sums;           // [sequence][part]: of r
+  double* sums;           // [sequence][chunk]: of r
   uint32_t* done;         // [sequence]: parts that are done; 0 before and after
   int64_t p_sb, p_sr, q_sb, q_sr, t_sb, u_sb;
   int batch, n, V, parts, part;       // `part` entries a part, a multiple of DR_STEP
+  int chunks;
 };
 
-// What counts as a probability: a positive number, otherwise 0.
-__device__ __forceinline__ float dr_clean(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+// What counts as a probability: NaN and what is below 0 as 0, infinity as the largest float.
+__device__ __forceinline__ float dr_clean(float x) { return __builtin_amdgcn_fmed3f(x, 0.f, 3.40282347e38f); }
 
+// A lane's entries of the chunk at c: c + (64 l + lane) * VE + 0 .. VE - 1 for l = 0 .. LOADS - 1, as they lie in
+// memory, zeros past V.
+template <typename IO>
+struct DraftWords {
+  static constexpr int VE = 16 / sizeof(typename IO::raw), LOADS = DR_PER / VE;
+  u32x4 w[LOADS];
+  __device__ __forceinline__ void load(const typename IO::raw* x, int c, int V) {
+    const int lane = threadIdx.x & 63;
+    if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && c + DR_CHUNK <= V) {     // the same in every lane
+#pragma unroll
+      for (int l = 0; l < LOADS; ++l) w[l] = *reinterpret_cast<const u32x4*>(x + c + (64 * l + lane) * VE);
+      return;
+    }
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int at = c + (64 * l + lane) * VE;
+      typename IO::raw e[VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) e[i] = at + i < V ? x[at + i] : (typename IO::raw)0;
+      __builtin_memcpy(&w[l], e, 16);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    typename IO::raw e[VE];
+    __builtin_memcpy(e, &w[i / VE], 16);
+    return dr_clean(IO::get(e[i % VE]));
+  }
+};
+
+// The row that is drawn from: p less q, or p but for one entry.
 template <typename IO>
 struct DraftRow {
   const typename IO::raw* p;
   const typename IO::raw* q;    // null: nothing to take off but `without`
   int without;                  // an entry that counts 0, or -1
-};
-
-// Entries c + (l * DR_THREADS + tid) * VE + 0 .. VE - 1 of a row for l = 0 .. DR_PER / VE - 1.
-template <typename IO>
-__device__ __forceinline__ void dr_load(const typename IO::raw* x, int c, int V, float* f) {
-  typedef typename IO::raw raw;
-  constexpr int VE = 16 / sizeof(raw);
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  struct Step {
+    DraftWords<IO> p, q;
+  };
+  __device__ __forceinline__ void load(Step& S, int c, int V) const {
+    S.p.load(p, c, V);
+    if (q) S.q.load(q, c, V);
+  }
+  __device__ __forceinline__ void rest(const Step& S, int c, double* r) const {
+    constexpr int VE = DraftWords<IO>::VE;
+    if (q) {
 #pragma unroll
-  for (int l = 0; l < DR_PER / VE; ++l) {
-    const int at = c + (l * DR_THREADS + (int)threadIdx.x) * VE;
-    if (vec && at + VE <= V) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(x + at);
-      raw e[VE];
-      __builtin_memcpy(e, &w, 16);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) f[l * VE + i] = dr_clean(IO::get(e[i]));
+      for (int i = 0; i < DR_PER; ++i) {
+        const float x = S.q.get(i);
+        r[i] = (double)fmaxf(S.p.get(i), x) - (double)x;
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) f[l * VE + i] = at + i < V ? dr_clean(IO::get(x[at + i])) : 0.f;
+      for (int i = 0; i < DR_PER; ++i)
+        r[i] = c + (64 * (i / VE) + (int)(threadIdx.x & 63)) * VE + i % VE == without ? 0.0 : (double)S.p.get(i);
     }
   }
-}
-
-// r of these entries; `all`: of p alone.
-template <typename IO>
-__device__ __forceinline__ void dr_rest(const DraftRow<IO>& R, int c, int V, bool all, double* r) {
-  constexpr int VE = 16 / sizeof(typename IO::raw);
-  float f[DR_PER], g[DR_PER];
-  dr_load<IO>(R.p, c, V, f);
-  if (R.q && !all) {
-    dr_load<IO>(R.q, c, V, g);
-#pragma unroll
-    for (int i = 0; i < DR_PER; ++i) r[i] = fmax((double)f[i] - (double)g[i], 0.0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < DR_PER; ++i) {
-      const int at = c + (i / VE * DR_THREADS + (int)threadIdx.x) * VE + i % VE;
-      r[i] = at == R.without && !all ? 0.0 : (double)f[i];
-    }
-  }
-}
+};
 
 __device__ __forceinline__ double dr_shfl_up(double v, int o) { return __shfl_up(v, o, 64); }
 __device__ __forceinline__ double dr_scan(double v) {           // inclusive, over the wavefront
@@ -103,9 +115,7 @@ template <typename IO>
 __global__ __launch_bounds__(DR_THREADS) void verify_drafts_kernel(const DraftArgs A) {
   typedef typename IO::raw raw;
   constexpr int VE = 16 / sizeof(raw), LOADS = DR_PER / VE;
-  __shared__ double waves[DR_THREADS / 64], totals[LOADS][DR_THREADS / 64];
   __shared__ uint32_t last;
-  __shared__ int found;
   const int b = blockIdx.x / A.parts, part = blockIdx.x - b * A.parts;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const raw* const p = reinterpret_cast<const raw*>(A.p) + b * A.p_sb;
@@ -142,145 +152,122 @@ __global__ __launch_bounds__(DR_THREADS) void verify_drafts_kernel(const DraftAr
     R.without = t >= 0 && t < A.V ? (int)t : -1;
   }
 
-  // over the workgroup, the same in every thread
-  auto block_sum = [&](double v) {
-    v = dr_sum(v);
-    if (lane == 0) waves[wave] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < DR_THREADS / 64; ++w) v += waves[w];
-    __syncthreads();
-    return v;
-  };
-  auto range_sum = [&](int lo, int hi, bool all) {
-    double v = 0.0;
-    for (int c = lo; c < hi; c += DR_STEP) {
-      double r[DR_PER];
-      dr_rest<IO>(R, c, A.V, all, r);
+  // The wavefront's chunks lo, lo + by .. of W; the entries of one are on their way while those of the one before are
+  // added.
+  auto sum_chunks = [&](const DraftRow<IO>& W, int lo, int hi, int by, auto done) {
+    typename DraftRow<IO>::Step now, next;
+    W.load(now, lo, A.V);
+    for (int c = lo; c < hi; c += by) {
+      if (c + by < hi) W.load(next, c + by, A.V);
+      double r[DR_PER], v = 0.0;
+      W.rest(now, c, r);
 #pragma unroll
       for (int i = 0; i < DR_PER; ++i) v += r[i];
+      done(c, dr_sum(v));
+      now = next;
     }
-    return block_sum(v);
   };
-  const double mine = range_sum(part * A.part, min(A.V, (part + 1) * A.part), false);
-  double* const sums = A.sums + (int64_t)b * A.parts;
-  if (tid == 0) {
-    __hip_atomic_store(sums + part, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    last = __hip_atomic_fetch_add(A.done + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(A.parts - 1);
-  }
+  double* const sums = A.sums + (int64_t)b * A.chunks;
+  auto put = [&](int c, double v) {
+    if (lane == 0) __hip_atomic_store(sums + c / DR_CHUNK, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  const int begin = part * A.part + wave * DR_CHUNK, end = min(A.V, (part + 1) * A.part);
+  if (begin < end) sum_chunks(R, begin, end, DR_STEP, put);
+  // Sums go to memory past the caches that other XCDs do not see, are waited for before the count goes up, and are
+  // read past them too: nothing else that another workgroup wrote is read, so no cache is emptied (which costs
+  // 10 us where 128 sequences end while others still read: 46 -> 36).
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (!last) return;
-  if (tid == 0) __hip_atomic_store(A.done + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  if (tid == 0) last = __hip_atomic_fetch_add(A.done + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(A.parts - 1);
+  __syncthreads();
+  if (!last || wave != 0) return;
+  if (lane == 0) __hip_atomic_store(A.done + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
-  // the part: every wavefront looks for itself, 64 parts a round
-  auto part_sum = [&](int i) {
-    return i < A.parts ? __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+  auto chunk_sum = [&](int i) {
+    return i < A.chunks ? __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
   };
-  double total = 0.0;
-  for (int i = 0; i < A.parts; i += 64) total += __shfl(dr_scan(part_sum(i + lane)), 63, 64);
+  auto total_of = [&]() {
+    double v = 0.0;
+    for (int i = 0; i < A.chunks; i += 64) v += __shfl(dr_scan(chunk_sum(i + lane)), 63, 64);
+    return v;
+  };
   const double drawn = fmax((double)u[A.n], 0.0);
-  int lo = 0, hi = 0;                                          // where the entry is
+  double total = total_of();
+  if (!(total > 0.0)) {
+    // Nothing is left (p below q at every entry but for rounding): p's own row, which this wavefront sums alone.
+    R.q = nullptr;
+    R.without = -1;
+    sum_chunks(R, 0, A.V, DR_CHUNK, put);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    total = total_of();
+  }
+  const double target = drawn * total;
+  int pick = -1, at = -1;
   double before = 0.0;
-  const bool all = !(total > 0.0);
-  if (all) {
-    // Nothing is left (p below q at every entry but for rounding): p's own row, which this workgroup reads alone.
-    total = range_sum(0, A.V, true);
-    hi = total > 0.0 ? A.V : 0;
-  } else {
-    int at = -1;
-    bool passed = false;
-    for (int i = 0; i < A.parts; i += 64) {
-      const double v = part_sum(i + lane), upto = before + dr_scan(v);
-      const uint64_t pass = __ballot(upto > drawn * total && v > 0.0), some = __ballot(v > 0.0);
-      if (pass) {
-        const int k = __builtin_ctzll(pass);
-        at = i + k;
-        before = __shfl(upto - v, k, 64);
-        passed = true;
-        break;
-      }
+  bool passed = false;
+  for (int i = 0; i < A.chunks && !passed; i += 64) {
+    const double v = chunk_sum(i + lane), upto = before + dr_scan(v);
+    const uint64_t pass = __ballot(upto > target && v > 0.0), some = __ballot(v > 0.0);
+    passed = pass != 0;
+    if (passed) {
+      at = i + __builtin_ctzll(pass);
+      before = __shfl(upto - v, at - i, 64);
+    } else {
       if (some) at = i + 63 - __builtin_clzll(some);           // u so near 1 that no sum passes: the last one
       before = __shfl(upto, 63, 64);
     }
-    if (!passed) before = -INFINITY;                           // nor does one of its entries
-    lo = at * A.part;
-    hi = min(A.V, lo + A.part);
   }
-  const double target = drawn * total;
-  if (tid == 0) found = -1;
-  __syncthreads();
-  if (hi > lo) {
+  if (at >= 0) {
+    const int c = at * DR_CHUNK;
+    double r[DR_PER], run = passed ? before : -INFINITY;       // where no sum passes, none of its entries does
+    typename DraftRow<IO>::Step S;
+    R.load(S, c, A.V);
+    R.rest(S, c, r);
     int best = -1;                                             // the last entry that is not 0
-    for (int c = lo; c < hi; c += DR_STEP) {
-      double r[DR_PER], s[LOADS], upto[LOADS];
-      dr_rest<IO>(R, c, A.V, all, r);
+    bool found = false;
 #pragma unroll
-      for (int l = 0; l < LOADS; ++l) {
-        s[l] = 0.0;
+    for (int l = 0; l < LOADS; ++l) {
+      double s = 0.0;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          s[l] += r[l * VE + e];
-          if (r[l * VE + e] > 0.0) best = c + (l * DR_THREADS + tid) * VE + e;
-        }
-        upto[l] = dr_scan(s[l]);
-        if (lane == 63) totals[l][wave] = upto[l];
+      for (int e = 0; e < VE; ++e) s += r[l * VE + e];
+      const double upto = dr_scan(s);
+      const uint64_t pass = __ballot(run + upto > target && s > 0.0);
+      int index = -1;                                          // the lane's entry that passes, or its last
+      double t = run + (upto - s);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        if (r[l * VE + e] > 0.0 && (index < 0 || !pass || t <= target)) index = c + (64 * l + lane) * VE + e;
+        t += r[l * VE + e];
       }
-      __syncthreads();
-      double run = before;
-      int hit = -1;
-#pragma unroll
-      for (int l = 0; l < LOADS; ++l)
-        for (int w = 0; w < DR_THREADS / 64; ++w) {
-          const double v = totals[l][w];
-          if (hit < 0 && w == wave) {
-            const uint64_t pass = __ballot(run + upto[l] > target && s[l] > 0.0);
-            if (pass) {
-              const int k = __builtin_ctzll(pass);
-              if (lane == k) {
-                double t = run + (upto[l] - s[l]);
-                int index = -1;
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                  const bool take = r[l * VE + e] > 0.0 && (index < 0 || t <= target);
-                  if (take) index = c + (l * DR_THREADS + tid) * VE + e;
-                  t += r[l * VE + e];
-                }
-                hit = index;
-              }
-              hit = __shfl(hit, k, 64);
-            }
-          }
-          run += v;
-        }
-      // the first wavefront's hit, in the order of the entries
-      if (hit >= 0 && lane == 0) atomicMin(reinterpret_cast<unsigned int*>(&found), (unsigned)hit);
-      __syncthreads();
-      if (found >= 0) break;
-      before = run;
+      if (!found && pass) {
+        found = true;
+        pick = __shfl(index, __builtin_ctzll(pass), 64);
+      }
+      best = max(best, index);
+      run += __shfl(upto, 63, 64);
     }
-    if (found < 0) {                                           // uniform: read after a barrier
-      __syncthreads();
-      if (best >= 0) atomicMax(&found, best);
-      __syncthreads();
+    if (!found) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
+      pick = best;
     }
   }
-  const int pick = found;
-  for (int i = tid; i <= A.n; i += DR_THREADS)
+  for (int i = lane; i <= A.n; i += 64)
     A.out[(int64_t)b * (A.n + 1) + i] = i < accepted ? tokens[i] : i == accepted ? pick : -1;
-  if (tid == 0) A.accepted[b] = accepted;
+  if (lane == 0) A.accepted[b] = accepted;
 }
 
-// Parts of a row: as many as give 6 workgroups a CU, of whole steps.
+// Parts of a row: as many as give 8 workgroups a CU, of whole steps.
 static void dr_plan(int64_t batch, int64_t V, int64_t* parts, int64_t* part) {
   const int64_t steps = (V + DR_STEP - 1) / DR_STEP;
-  int64_t n = (6 * (int64_t)device_cu_count() + batch - 1) / batch;
+  int64_t n = (8 * (int64_t)device_cu_count() + batch - 1) / batch;
   if (n > steps) n = steps;
   const int64_t per = (steps + n - 1) / n;
   *part = per * DR_STEP;
   *parts = (steps + per - 1) / per;
 }
+
+static int64_t dr_chunks(int64_t V) { return (V + DR_CHUNK - 1) / DR_CHUNK; }
 
 }  // namespace pp
 
@@ -288,9 +275,7 @@ using namespace pp;
 
 extern "C" int64_t pp_verify_drafts_workspace_size(int64_t batch, int64_t V) {
   if (batch <= 0 || V <= 0) return 0;
-  int64_t parts, part;
-  dr_plan(batch, V, &parts, &part);
-  return batch * parts * 8;
+  return batch * dr_chunks(V) * 8;
 }
 
 extern "C" int pp_verify_drafts(const void* target, int64_t p_sb, int64_t p_sr, const void* draft, int64_t q_sb,
@@ -309,12 +294,14 @@ extern "C" int pp_verify_drafts(const void* target, int64_t p_sb, int64_t p_sr, 
   int64_t parts, part;
   dr_plan(batch, V, &parts, &part);
   PP_REQUIRE(batch * parts <= INT32_MAX, "pp_verify_drafts: too many sequences");
-  PP_REQUIRE(workspace && workspace_size >= batch * parts * 8 && aligned(workspace, 8),
-             "pp_verify_drafts: workspace of %lld bytes at an 8-byte boundary needed", (long long)(batch * parts * 8));
+  const int64_t need = batch * dr_chunks(V) * 8;
+  PP_REQUIRE(workspace && workspace_size >= need && aligned(workspace, 8),
+             "pp_verify_drafts: workspace of %lld bytes at an 8-byte boundary needed", (long long)need);
   PP_REQUIRE(done && done_size >= 4 * batch && aligned(done, 4), "pp_verify_drafts: %lld bytes of counts, zero, needed",
              (long long)(4 * batch));
   const DraftArgs A{target, n ? draft : nullptr, tokens, uniforms, counts, out, accepted, (double*)workspace, (uint32_t*)done,
-                    p_sb, p_sr, q_sb, q_sr, t_sb, u_sb, (int)batch, (int)n, (int)V, (int)parts, (int)part};
+                    p_sb, p_sr, q_sb, q_sr, t_sb, u_sb, (int)batch, (int)n, (int)V, (int)parts, (int)part,
+                    (int)dr_chunks(V)};
   auto kern = dtype == PP_F16 ? verify_drafts_kernel<IoF16>
               : dtype == PP_BF16 ? verify_drafts_kernel<IoBf16> : verify_drafts_kernel<IoF32>;
   hipLaunchKernelGGL(kern, dim3((unsigned)(batch * parts)), dim3(DR_THREADS), 0, (hipStream_t)stream, A);

@@ -27,9 +27,9 @@ def verify_drafts(target, draft, tokens, uniforms, counts=None):
     Draft i is kept while ``u_i q_i(token) < p_i(token)``.  The token after the kept ones is drawn with ``u_n``: at a
     refused draft from ``max(p_i - q_i, 0)`` (``draft=None``: from p_i without the token; from p_i where nothing is left),
     after the last from ``p_count``; it is the first whose sum of entries up to it passes ``u_n`` times the sum of all.  So
-    the answer is distributed as the target's own.  Sums are held in float64; rows need not add up to one.  An entry that is
-    not a positive finite number counts as 0, as does a token outside [0, V); from a row of nothing else the token is
-    -1.  With n = 0 it draws a token from each row.
+    the answer is distributed as the target's own.  Sums are held in float64; rows need not add up to one.  A NaN or an
+    entry below 0 counts as 0, infinity as the largest float32, a token outside [0, V) has probability 0; from a row of
+    nothing the token is -1.  With n = 0 it draws a token from each row.
 
     Nothing waits for the device, and a call can be captured in a HIP graph.  There is no backward pass.
     """

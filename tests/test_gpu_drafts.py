@@ -16,8 +16,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
 def clean(x):
-    x = x.double()
-    return torch.where((x > 0) & x.isfinite(), x, 0.0)
+    return x.double().nan_to_num(0.0).clamp(0.0, torch.finfo(torch.float32).max)
 
 
 def plain(p, q, tokens, u, counts=None):
