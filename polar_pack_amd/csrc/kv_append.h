@@ -68,20 +68,21 @@ __device__ __forceinline__ Unit kv_unit(const KvCache& C) {
 
 // Codes and scale of one page, head and side (8 bits): thread (tg, dg) holds the values of tokens 4 tg .. 4 tg + 3 and
 // d 8 dg .. 8 dg + 7, value(i, j).  `top`: the thread's largest magnitude, of which bits(top) are the word as
-// a float; any order-keeping words do for the maximum.  red is 16 words of LDS, tile D * (block / 4 + 1) for V.
+// a float; any order-keeping words do for the maximum.  red is 16 words of LDS, tile D * (block / 4 + 1) for V.  The page is
+// that of threads tid = 0 .. nthr - 1, whole wavefronts, of a workgroup whose other threads make the same call for other
+// heads; not `active`: for none.
 template <int CODES, int D, typename B, typename V>
 __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, int head, int isv, uint32_t top, B bits_of,
-                                            uint32_t* red, uint32_t* tile, V value) {
+                                            uint32_t* red, uint32_t* tile, int tid, int nthr, bool active, V value) {
   using Q = KvCodes<CODES>;
-  const int tid = threadIdx.x, nthr = blockDim.x;
   const int held = P.lo, end = P.hi;                   // new tokens held..end-1 of the page
   const int tg = tid / (D / 8), dg = tid % (D / 8);
-  const bool mine = tid < (C.block / 4) * (D / 8);
+  const bool mine = active && tid < (C.block / 4) * (D / 8);
   top = wave_umax(top);
   if ((tid & 63) == 0) red[tid >> 6] = top;
   const int64_t ph = (int64_t)P.page * C.heads + head;
   float* scale_at = (isv ? C.vs : C.ks) + ph;
-  const float was = held ? *scale_at : 0.f;
+  const float was = held && active ? *scale_at : 0.f;
   __syncthreads();
   for (int w = 0; w < (nthr + 63) / 64; ++w) top = max(top, red[w]);
   top = bits_of(top);
@@ -95,7 +96,7 @@ __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, in
   // qmax / max|x| is rounded once, 1 / scale of a rounded scale twice: half as many codes on the wrong
   // side of a tie
   const float inv = !finite ? 0.f : need == bits ? Q::kMax / __uint_as_float(top) : 1.0f / now;
-  if (tid == 0) *scale_at = now;
+  if (tid == 0 && active) *scale_at = now;
 
   uint32_t w8[4][2];
 #pragma unroll
@@ -120,7 +121,7 @@ __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, in
         if (t >= held && t < end) *reinterpret_cast<u32x2*>(k + t * D + 8 * dg) = u32x2{w8[i][0], w8[i][1]};
       }
     }
-    if (grown)
+    if (grown && active)
       for (int w = tid; w < held * (D / 4); w += nthr) {
         uint32_t* p = reinterpret_cast<uint32_t*>(k) + w;
         *p = rescale(*p);
@@ -139,6 +140,7 @@ __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, in
     }
   }
   __syncthreads();
+  if (!active) return;
   uint32_t* v = reinterpret_cast<uint32_t*>(C.v + base);
   const int wl = C.shift - 2, words = D << wl;
   if (held == 0 && end == C.block) {                   // all new: whole 16-byte pieces
@@ -170,8 +172,9 @@ __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, in
 // The 16-bit values of a piece that thread (tg, dg) holds, zeros where there are none, and the largest word of
 // magnitudes: those of 16-bit values are ordered like their words, NaN last.
 template <int D>
-__device__ __forceinline__ uint32_t load_unit(const Piece& P, const uint16_t* src, int64_t st, int vec, bool mine, u32x4* x) {
-  const int tg = threadIdx.x / (D / 8), dg = threadIdx.x % (D / 8);
+__device__ __forceinline__ uint32_t load_unit(const Piece& P, const uint16_t* src, int64_t st, int vec, int tid, bool mine,
+                                              u32x4* x) {
+  const int tg = tid / (D / 8), dg = tid % (D / 8);
   u16x2 big = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -66,10 +66,11 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const AppendArgs A) {
   __shared__ uint32_t red[16];
   extern __shared__ uint32_t tile[];                   // V codes: [D][block / 4 + 1] words
   u32x4 x[4];
-  const uint32_t top = load_unit<D>(P, A.x[isv] + (int64_t)head * A.sh[isv], A.st[isv], A.vec,
-                                    (int)threadIdx.x < (C.block / 4) * (D / 8), x);
-  append_page<CODES, D>(C, P, head, isv, top, [](uint32_t w) { return mag(IO::get((uint16_t)w)); }, red, tile,
-                        [&](int i, int j) { return half_of<IO>(x[i], j); });
+  const int tid = threadIdx.x;
+  const uint32_t top = load_unit<D>(P, A.x[isv] + (int64_t)head * A.sh[isv], A.st[isv], A.vec, tid,
+                                    tid < (C.block / 4) * (D / 8), x);
+  append_page<CODES, D>(C, P, head, isv, top, [](uint32_t w) { return mag(IO::get((uint16_t)w)); }, red, tile, tid,
+                        blockDim.x, true, [&](int i, int j) { return half_of<IO>(x[i], j); });
 }
 
 // Reading back: the same units, each output row written once; tokens that lie on no page, or past

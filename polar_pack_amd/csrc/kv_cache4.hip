@@ -1,7 +1,7 @@
 // The 4-bit cache: appending to it, as the values are or turned, and reading it back.
 //
-// A workgroup takes 32 tokens of a page (16 where a page is no longer) and one or more heads, keys and values both:
-// a value of either that is not finite marks the token in the scales of its keys.  Thread (tg, dg) holds tokens
+// A workgroup takes 32 tokens of a page (16 where a page is no longer) and a head, or several side by side, keys and values
+// both: a value of either that is not finite marks the token in the scales of its keys.  Thread (tg, dg) holds tokens
 // 4 tg .. 4 tg + 3 and values 8 dg .. 8 dg + 7, so the largest of a group of 32 meets over four neighbouring lanes.
 // Turned keys are computed in 64 bits and rounded to odd, so that a code is the one nearest to the key whatever lies
 // between: a step of 4 bits is wide, and a rounding before it would move one value in some 10^7 by a whole step.
@@ -17,8 +17,8 @@ struct Append4Args {
   AppendArgs A;
   Rot R;
   RotRows Q;
-  int per, chunks;
-  unsigned units;
+  int beside, chunks, threads;   // heads a workgroup, workgroups a piece, threads a head
+  Roles roles;
 };
 
 // A number of 64 bits as a float, rounded to odd: what is compared or rounded again to fewer bits comes out as if
@@ -41,122 +41,123 @@ constexpr int ROW4 = 20;      // bytes of a row of V codes in LDS: 32 tokens, an
 
 // TURN: keys are turned (in 64 bits).
 template <typename IO, int D, bool TURN>
-__global__ __launch_bounds__(256) void kv_append4_kernel(const Append4Args X) {
+__global__ __launch_bounds__(TURN ? 512 : 256, TURN ? 3 : 4) void kv_append4_kernel(const Append4Args X) {
   typedef std::conditional_t<TURN, double, float> real;
-  if (TURN && blockIdx.x >= X.units) {
-    rotate_queries<IO>(X.A.S, X.R, X.Q, blockIdx.x - X.units);
+  unsigned index = blockIdx.x;
+  if (TURN && !X.roles.appends(blockIdx.x, index)) {
+    rotate_queries<IO>(X.A.S, X.R, X.Q, index);
     return;
   }
   const AppendArgs& A = X.A;
   const KvCache& C = A.C;
-  const int item = blockIdx.x / X.chunks, h0 = (blockIdx.x - item * X.chunks) * X.per, h1 = min(h0 + X.per, C.heads);
+  const int item = index / X.chunks, sub = TURN ? uniform(threadIdx.x / X.threads) : 0;
+  const int tid = threadIdx.x - sub * X.threads, nthr = X.threads, head = (index - item * X.chunks) * X.beside + sub;
   const int shift = shift4(C);
   Piece P;
   if (!kv_piece(C, A.S, item, shift, P) || P.page < 0) return;
-  __shared__ __align__(16) uint8_t tile[D * ROW4];
-  __shared__ uint32_t bad[2];                            // tokens that are not finite, of this head and the next
-  extern __shared__ __align__(16) uint8_t table[];
-  Trig<real>* const tab = reinterpret_cast<Trig<real>*>(table);
-  const int tid = threadIdx.x, nthr = blockDim.x;
+  __shared__ uint32_t bad[8];                            // tokens that are not finite, for each head
+  extern __shared__ __align__(16) uint8_t lds[];         // V codes of each head, then the table
+  uint8_t* const tile = lds + sub * (D * ROW4);
   const int tg = tid / (D / 8), dg = tid % (D / 8);
-  const bool mine = tid < (1 << shift) / 4 * (D / 8), leads = mine && dg % 4 == 0;
-  if (tid < 2) bad[tid] = 0;
+  const bool active = head < C.heads, mine = active && tid < (1 << shift) / 4 * (D / 8), leads = mine && dg % 4 == 0;
+  if (tid == 0) bad[sub] = 0;
+  Trig<real>* const tab = reinterpret_cast<Trig<real>*>(lds + X.beside * (D * ROW4));
   if constexpr (TURN) rot_table(X.R, P, tab);
   __syncthreads();
-  for (int head = h0; head < h1; ++head) {
-    uint32_t& flags = bad[head & 1];
-    u32x4 xv[4];
-    load_unit<D>(P, A.x[1] + (int64_t)head * A.sh[1], A.st[1], A.vec, mine, xv);
-    real xk[4][8];
-    if constexpr (TURN) {
-      load_turned<IO, real, D>(X.R, P, A.x[0] + (int64_t)head * A.sh[0], A.st[0], A.vec, mine, tab, xk);
-    } else {
-      u32x4 w[4];
-      load_unit<D>(P, A.x[0] + (int64_t)head * A.sh[0], A.st[0], A.vec, mine, w);
+  uint32_t& flags = bad[sub];
+  u32x4 xv[4];
+  load_unit<D>(P, A.x[1] + (int64_t)head * A.sh[1], A.st[1], A.vec, tid, mine, xv);
+  uint32_t kw[4], kb[4], vb = 0, lost = 0;
+  auto code_keys = [&](int i, const real* x) {
+    float f[8];
+    uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xk[i][j] = half_of<IO>(w[i], j);
+    for (int j = 0; j < 8; ++j) {
+      f[j] = odd_float(x[j]);
+      top = max(top, mag(f[j]));
     }
-    uint32_t kw[4], kb[4], vb = 0, lost = 0;
-    float f[4][8];
+    lost |= top >= 0x7f800000u ? 1u << i : 0u;
+    const int e = scale4(quad_max(top));
+    const float s = scale4_value(e);
+    kb[i] = scale4_byte(e);
+    kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], s, 0);
+    kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[2], f[3], s, 1);
+    kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[4], f[5], s, 2);
+    kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[6], f[7], s, 3);
+  };
+  const uint16_t* const keys = A.x[0] + (int64_t)head * A.sh[0];
+  if constexpr (TURN) {
+    load_turned<IO, real, D>(X.R, P, keys, A.st[0], A.vec, tid, mine, tab, code_keys);
+  } else {
+    u32x4 w[4];
+    load_unit<D>(P, keys, A.st[0], A.vec, tid, mine, w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t top = 0;
+      real x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f[i][j] = odd_float(xk[i][j]);
-        top = max(top, mag(f[i][j]));
-      }
-      lost |= top >= 0x7f800000u ? 1u << i : 0u;
-      const int e = scale4(quad_max(top));
-      const float s = scale4_value(e);
-      kb[i] = scale4_byte(e);
-      kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[i][0], f[i][1], s, 0);
-      kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[i][2], f[i][3], s, 1);
-      kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[i][4], f[i][5], s, 2);
-      kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[i][6], f[i][7], s, 3);
+      for (int j = 0; j < 8; ++j) x[j] = half_of<IO>(w[i], j);
+      code_keys(i, x);
     }
-    // a byte of V is two tokens of different scales: they are divided out first, exactly
+  }
+  float f[4][8];
+  // a byte of V is two tokens of different scales: they are divided out first, exactly
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u16x2 big = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, xv[i][j] & 0x7fff7fffu));
+    const uint32_t top = mag(IO::get((uint16_t)max((uint32_t)big[0], (uint32_t)big[1])));
+    lost |= top >= 0x7f800000u ? 1u << i : 0u;
+    const int e = scale4(quad_max(top));
+    const float s = scale4_value(-e);
+    vb |= scale4_byte(e) << (8 * i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[i][j] = half_of<IO>(xv[i], j) * s;
+  }
+  if (mine) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0][j], f[1][j], 1.f, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2][j], f[3][j], 1.f, 1);
+      *reinterpret_cast<uint16_t*>(tile + (8 * dg + j) * ROW4 + 2 * tg) = (uint16_t)w;
+    }
+    if (lost) atomicOr(&flags, lost << (4 * tg));
+  }
+  __syncthreads();
+  if (!active) return;
+  const uint32_t broken = flags;
+  const int64_t ph = (int64_t)P.page * C.heads + head;
+  if (mine) {
+    const int64_t row = ph * C.block + P.from;
+    uint8_t* const vs = scales_v(C) + (ph * (D / 32) + dg / 4) * C.block + P.from + 4 * tg;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u16x2 big = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, xv[i][j] & 0x7fff7fffu));
-      const uint32_t top = mag(IO::get((uint16_t)max((uint32_t)big[0], (uint32_t)big[1])));
-      lost |= top >= 0x7f800000u ? 1u << i : 0u;
-      const int e = scale4(quad_max(top));
-      const float s = scale4_value(-e);
-      vb |= scale4_byte(e) << (8 * i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = half_of<IO>(xv[i], j) * s;
-    }
-    if (mine) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0][j], f[1][j], 1.f, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2][j], f[3][j], 1.f, 1);
-        *reinterpret_cast<uint16_t*>(tile + (8 * dg + j) * ROW4 + 2 * tg) = (uint16_t)w;
-      }
-      if (lost) atomicOr(&flags, lost << (4 * tg));
-    }
-    __syncthreads();
-    const uint32_t broken = flags;
-    if (tid == 0) bad[(head + 1) & 1] = 0;
-    const int64_t ph = (int64_t)P.page * C.heads + head;
-    if (mine) {
-      const int64_t row = ph * C.block + P.from;
-      uint8_t* const vs = scales_v(C) + (ph * (D / 32) + dg / 4) * C.block + P.from + 4 * tg;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 4 * tg + i;
-        if (t < P.lo || t >= P.hi) continue;
-        *reinterpret_cast<uint32_t*>(C.k + (row + t) * (D / 2) + 4 * dg) = kw[i];
-        if (leads) {
-          scales_k(C)[(row + t) * (D / 32) + dg / 4] = (uint8_t)(broken >> t & 1 ? SCALE4_NAN : kb[i]);
-          vs[i] = (uint8_t)(vb >> (8 * i));
-        }
+      const int t = 4 * tg + i;
+      if (t < P.lo || t >= P.hi) continue;
+      *reinterpret_cast<uint32_t*>(C.k + (row + t) * (D / 2) + 4 * dg) = kw[i];
+      if (leads) {
+        scales_k(C)[(row + t) * (D / 32) + dg / 4] = (uint8_t)(broken >> t & 1 ? SCALE4_NAN : kb[i]);
+        vs[i] = (uint8_t)(vb >> (8 * i));
       }
     }
-    uint8_t* const v = C.v + ph * (D / 2) * C.block + P.from / 2;
-    const int row_bytes = C.block / 2;
-    if (P.lo == 0 && P.hi == 32) {
-      for (int d = tid; d < D; d += nthr) {
-        const uint32_t* t = reinterpret_cast<const uint32_t*>(tile + d * ROW4);
-        *reinterpret_cast<u32x4*>(v + d * row_bytes) = u32x4{t[0], t[1], t[2], t[3]};
-      }
-    } else {
-      const int wl = shift - 3;                          // words of 8 tokens; other tokens' codes stay
-      for (int w = tid; w < D << wl; w += nthr) {
-        const int d = w >> wl, q = w & ((1 << wl) - 1), lo = max(P.lo - 8 * q, 0), hi = min(P.hi - 8 * q, 8);
-        if (lo >= hi) continue;
-        uint32_t* const at = reinterpret_cast<uint32_t*>(v + d * row_bytes) + q;
-        const uint32_t out = *reinterpret_cast<const uint32_t*>(tile + d * ROW4 + 4 * q);
-        const uint32_t mask = (hi - lo == 8 ? ~0u : (1u << (4 * (hi - lo))) - 1) << (4 * lo);
-        *at = mask == ~0u ? out : (*at & ~mask) | (out & mask);
-      }
+  }
+  uint8_t* const v = C.v + ph * (D / 2) * C.block + P.from / 2;
+  const int row_bytes = C.block / 2;
+  if (P.lo == 0 && P.hi == 32) {
+    for (int d = tid; d < D; d += nthr) {
+      const uint32_t* t = reinterpret_cast<const uint32_t*>(tile + d * ROW4);
+      *reinterpret_cast<u32x4*>(v + d * row_bytes) = u32x4{t[0], t[1], t[2], t[3]};
     }
-    if (head + 1 < h1) __syncthreads();                  // LDS is read
+  } else {
+    const int wl = shift - 3;                          // words of 8 tokens; other tokens' codes stay
+    for (int w = tid; w < D << wl; w += nthr) {
+      const int d = w >> wl, q = w & ((1 << wl) - 1), lo = max(P.lo - 8 * q, 0), hi = min(P.hi - 8 * q, 8);
+      if (lo >= hi) continue;
+      uint32_t* const at = reinterpret_cast<uint32_t*>(v + d * row_bytes) + q;
+      const uint32_t out = *reinterpret_cast<const uint32_t*>(tile + d * ROW4 + 4 * q);
+      const uint32_t mask = (hi - lo == 8 ? ~0u : (1u << (4 * (hi - lo))) - 1) << (4 * lo);
+      *at = mask == ~0u ? out : (*at & ~mask) | (out & mask);
+    }
   }
 }
 
@@ -233,13 +234,15 @@ static unsigned threads4(const KvCache& C, int D) { return unit_threads(1 << shi
 int kv_append4(const AppendArgs& A, const Rot* rot, const RotRows* q, int D, int dtype, hipStream_t st) {
   const bool h = dtype == PP_F16;
   const int64_t items = kv_pieces(A.S, shift4(A.C));
-  const unsigned threads = threads4(A.C, D);
-  Append4Args X{A, rot ? *rot : Rot{}, q ? *q : RotRows{}, rot ? heads_per(items, A.C.heads) : 1, 0, 0};
-  X.chunks = (A.C.heads + X.per - 1) / X.per;
+  Append4Args X{A, rot ? *rot : Rot{}, q ? *q : RotRows{}, 1, 0, (int)threads4(A.C, D), Roles{}};
+  if (rot) X.beside = heads_beside(A.S, X.threads, A.C.heads);
+  X.chunks = (A.C.heads + X.beside - 1) / X.beside;
+  const unsigned threads = X.threads * X.beside;
   const int64_t units = items * X.chunks, blocks = units + (rot ? query_blocks(X.R, X.Q, threads) : 0);
   PP_REQUIRE(blocks <= UINT32_MAX / threads, "kv append: too many tokens and sequences");
-  X.units = (unsigned)units;
-  const unsigned lds = rot ? (A.S.cu ? 1u << shift4(A.C) : 1u) * (unsigned)rot->half * (unsigned)sizeof(Trig<double>) : 0;
+  X.roles = roles(units, blocks);
+  const unsigned table = rot ? (A.S.cu ? 1u << shift4(A.C) : 1u) * (unsigned)rot_stride(*rot) * (unsigned)sizeof(Trig<double>) : 0;
+  const unsigned lds = X.beside * (unsigned)(D * ROW4) + table;
   return by_width(D, [&](auto d) -> int {
     constexpr int W = decltype(d)::value;
     auto kern = rot ? (h ? kv_append4_kernel<IoF16, W, true> : kv_append4_kernel<IoBf16, W, true>)

@@ -9,50 +9,51 @@ struct RotateArgs {
   AppendArgs A;
   Rot R;
   RotRows Q;
-  int per, chunks, table;    // heads a workgroup, workgroups a page and side, whether there is a table
-  unsigned units;            // workgroups that append; the others turn queries
+  int beside, chunks, threads;   // heads a workgroup, workgroups a page and side, threads a head
+  Roles roles;
 };
 
 template <int CODES, typename IO, int D>
-__global__ __launch_bounds__(4 * D) void kv_rotate_append_kernel(const RotateArgs X) {
-  if (blockIdx.x >= X.units) {
-    rotate_queries<IO>(X.A.S, X.R, X.Q, blockIdx.x - X.units);
+__global__ __launch_bounds__(D < 128 ? 512 : 4 * D, 4) void kv_rotate_append_kernel(const RotateArgs X) {
+  unsigned index;
+  if (!X.roles.appends(blockIdx.x, index)) {
+    rotate_queries<IO>(X.A.S, X.R, X.Q, index);
     return;
   }
   const AppendArgs& A = X.A;
   const KvCache& C = A.C;
-  const uint32_t n = 2 * (uint32_t)X.chunks, item = blockIdx.x / n, r = blockIdx.x - item * n;
-  const int isv = r >= (uint32_t)X.chunks, h0 = (int)(isv ? r - X.chunks : r) * X.per, h1 = min(h0 + X.per, C.heads);
+  const uint32_t n = 2 * (uint32_t)X.chunks, item = index / n, r = index - item * n;
+  const int isv = r >= (uint32_t)X.chunks, sub = uniform(threadIdx.x / X.threads), tid = threadIdx.x - sub * X.threads;
+  const int head = (int)(isv ? r - X.chunks : r) * X.beside + sub;
   Piece P;
   if (!kv_piece(C, A.S, (int)item, C.shift, P) || P.page < 0) return;
-  __shared__ uint32_t red[16];
+  __shared__ uint32_t maxima[8][16];
   extern __shared__ __align__(16) uint32_t lds[];      // of keys the table, of values the codes
-  const bool mine = (int)threadIdx.x < (C.block / 4) * (D / 8);
-  Trig<float>* const tab = X.table ? reinterpret_cast<Trig<float>*>(lds) : nullptr;
-  if (!isv && tab) {
-    rot_table(X.R, P, tab);
-    __syncthreads();
+  const bool active = head < C.heads, mine = active && tid < (C.block / 4) * (D / 8);
+  uint32_t* const red = maxima[sub];
+  const uint16_t* src = A.x[isv] + (int64_t)head * A.sh[isv];
+  if (isv) {
+    u32x4 x[4];
+    const uint32_t top = load_unit<D>(P, src, A.st[1], A.vec, tid, mine, x);
+    append_page<CODES, D>(C, P, head, 1, top, [](uint32_t w) { return mag(IO::get((uint16_t)w)); }, red,
+                          lds + sub * D * (C.block / 4 + 1), tid, X.threads, active,
+                          [&](int i, int j) { return half_of<IO>(x[i], j); });
+    return;
   }
-  for (int head = h0; head < h1; ++head) {
-    const uint16_t* src = A.x[isv] + (int64_t)head * A.sh[isv];
-    if (isv) {
-      u32x4 x[4];
-      const uint32_t top = load_unit<D>(P, src, A.st[1], A.vec, mine, x);
-      append_page<CODES, D>(C, P, head, 1, top, [](uint32_t w) { return mag(IO::get((uint16_t)w)); }, red, lds,
-                            [&](int i, int j) { return half_of<IO>(x[i], j); });
-    } else {
-      float x[4][8];
-      load_turned<IO, float, D>(X.R, P, src, A.st[0], A.vec, mine, tab, x);
-      uint32_t top = 0;
+  Trig<float>* const tab = reinterpret_cast<Trig<float>*>(lds);
+  rot_table(X.R, P, tab);
+  __syncthreads();
+  float x[4][8];
+  uint32_t top = 0;
+  load_turned<IO, float, D>(X.R, P, src, A.st[0], A.vec, tid, mine, tab, [&](int i, const float* v) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, mag(x[i][j]));
-      append_page<CODES, D>(C, P, head, 0, top, [](uint32_t w) { return w; }, red, lds,
-                            [&](int i, int j) { return x[i][j]; });
+    for (int j = 0; j < 8; ++j) {
+      x[i][j] = v[j];
+      top = max(top, mag(v[j]));
     }
-    if (head + 1 < h1) __syncthreads();                // LDS is read
-  }
+  });
+  append_page<CODES, D>(C, P, head, 0, top, [](uint32_t w) { return w; }, red, lds, tid, X.threads, active,
+                        [&](int i, int j) { return x[i][j]; });
 }
 
 }  // namespace pp
@@ -77,23 +78,23 @@ extern "C" int pp_kv_rotate_append(const pp_kv_cache* cache, const void* q, int6
   if (X.Q.x) {
     PP_REQUIRE(q_out && aligned(q, 2) && aligned(q_out, 16), "pp_kv_rotate_append: queries or their output null or not aligned");
     X.Q.vec = aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0;
-    const int64_t groups = rot_groups(tokens * rot_units(X.R.half, D), q_heads);
+    const int64_t groups = rot_groups(tokens * rot_units(X.R.half, D), q_heads, 1024);
     X.Q.per = (int)((q_heads + groups - 1) / groups);
   }
   PP_REQUIRE(X.Q.x || q_heads == 0, "pp_kv_rotate_append: null queries");
   if (cache->codes == PP_KV_E2M1) return kv_append4(X.A, &X.R, &X.Q, D, dtype, (hipStream_t)stream);
   const KvCache& C = X.A.C;
   const int64_t items = kv_pieces(X.A.S, C.shift);
-  const dim3 wg(unit_threads(C.block, D));
-  X.per = heads_per(2 * items, C.heads);
-  X.chunks = (C.heads + X.per - 1) / X.per;
+  X.threads = (int)unit_threads(C.block, D);
+  X.beside = heads_beside(X.A.S, X.threads, C.heads);
+  X.chunks = (C.heads + X.beside - 1) / X.beside;
+  const dim3 wg(X.threads * X.beside);
   const int64_t units = items * 2 * X.chunks, blocks = units + query_blocks(X.R, X.Q, wg.x);
   PP_REQUIRE(blocks <= UINT32_MAX / wg.x, "pp_kv_rotate_append: too many tokens and sequences");
-  X.units = (unsigned)units;
+  X.roles = roles(units, blocks);
   // a piece of a call without cu is one token
-  const int64_t table_bytes = (cu ? C.block : 1) * (int64_t)X.R.half * (int64_t)sizeof(Trig<float>);
-  X.table = table_bytes <= ROT_TABLE_MAX;
-  const unsigned tile = tile_bytes(C.block, D), lds = X.table && table_bytes > tile ? (unsigned)table_bytes : tile;
+  const unsigned table_bytes = (cu ? C.block : 1) * (unsigned)rot_stride(X.R) * (unsigned)sizeof(Trig<float>);
+  const unsigned tiles = tile_bytes(C.block, D) * X.beside, lds = table_bytes > tiles ? table_bytes : tiles;
   return by_width(D, [&](auto d) -> int {
     constexpr int W = decltype(d)::value;
     const bool i8 = cache->codes == PP_KV_INT8, h = dtype == PP_F16;

@@ -75,9 +75,13 @@ __device__ __forceinline__ void turn_trig(uint64_t t, Trig<float>& o) {
   o.s = k & 2 ? -b : b;
 }
 
-__device__ __forceinline__ int64_t rot_position(const Rot& R, int f, int64_t token) {
-  const int64_t at = (R.axes ? min((int)R.axes[f], R.n_axes - 1) : 0) * R.pos_ld + token;
+// A token's position on an axis, below n_axes.
+__device__ __forceinline__ int64_t rot_load(const Rot& R, int axis, int64_t token) {
+  const int64_t at = axis * R.pos_ld + token;
   return R.wide ? reinterpret_cast<const int64_t*>(R.pos)[at] : reinterpret_cast<const int32_t*>(R.pos)[at];
+}
+__device__ __forceinline__ int64_t rot_position(const Rot& R, int f, int64_t token) {
+  return rot_load(R, R.axes ? min((int)R.axes[f], R.n_axes - 1) : 0, token);
 }
 
 template <typename T>
@@ -145,12 +149,28 @@ __device__ __forceinline__ void rotate_unit(const Rot& R, const RotRows& A, int 
   const int units = R.half / 8;
   int at0, at1;                   // the unit's two pieces of 8 values
   Trig<float> w[8];
-  if (u < units) {
+  if (u < units && R.pos && R.axes) {
+    // Up to four axes: the token's positions first, all at once, then a choice for each frequency.
+    at0 = R.neighbours ? 16 * u : 8 * u;
+    at1 = R.neighbours ? at0 + 8 : at0 + R.half;
+    int64_t p[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) p[a] = rot_load(R, min(a, R.n_axes - 1), token);
+    uint8_t axis[8];
+    __builtin_memcpy(axis, R.axes + 8 * u, 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int a = axis[i];
+      int64_t at = a == 0 ? p[0] : a == 1 ? p[1] : a == 2 ? p[2] : p[3];
+      if (R.n_axes > 4) at = rot_load(R, min(a, R.n_axes - 1), token);
+      w[i] = rot_trig<float>(R, 8 * u + i, at);
+    }
+  } else if (u < units) {
+    if (R.pos) own = rot_load(R, 0, token);
     at0 = R.neighbours ? 16 * u : 8 * u;
     at1 = R.neighbours ? at0 + 8 : at0 + R.half;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i] = rot_trig<float>(R, 8 * u + i, R.pos ? rot_position(R, 8 * u + i, token) : own);
+    for (int i = 0; i < 8; ++i) w[i] = rot_trig<float>(R, 8 * u + i, own);
   } else {
     at0 = 2 * R.half + 16 * (u - units);
     at1 = at0 + 8 < A.D ? at0 + 8 : at0;
@@ -190,10 +210,12 @@ __device__ __forceinline__ void rotate_unit(const Rot& R, const RotRows& A, int 
 }
 
 // Host side.
-// Threads that share a unit's heads: as many as make 1024 threads a CU, since a thread's sines and cosines
-// cost as much as two or three heads.
-inline int64_t rot_groups(int64_t units, int64_t heads) {
-  const int64_t want = ((int64_t)device_cu_count() * 1024 + units - 1) / units;
+// Threads that share a unit's heads: as many as make `threads` a CU, since a thread's sines and cosines cost as much as
+// two or three heads.  512 where rows are all there is (16,200 tokens of 18 heads of 128: 26.7 us, with 1024 27.5); 1024
+// beside an append (16 ragged prompts of 32 query heads 99.9 us, with 512 104.9, with 4096 102.7; 4 prompts of 16 27.1,
+// 26.9, 35.3).
+inline int64_t rot_groups(int64_t units, int64_t heads, int threads) {
+  const int64_t want = ((int64_t)device_cu_count() * threads + units - 1) / units;
   return want < 1 ? 1 : want < heads ? want : heads;
 }
 int rot_check(const pp_rotary* r, const void* positions, int64_t pos_ld, int pos_type, int64_t tokens, int64_t head_dim,
