@@ -291,6 +291,21 @@ __device__ __forceinline__ float sum_halves(float v) {
 template <int I>
 using Int = std::integral_constant<int, I>;
 
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+  (f(Int<I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(std::make_integer_sequence<int, N>(), f);
+}
+
+// Byte t of four e5m2 numbers.
+__device__ __forceinline__ float bf8_byte(uint32_t w, int t) {
+  return t == 0 ? __builtin_amdgcn_cvt_f32_bf8(w, 0) : t == 1 ? __builtin_amdgcn_cvt_f32_bf8(w, 1)
+         : t == 2 ? __builtin_amdgcn_cvt_f32_bf8(w, 2) : __builtin_amdgcn_cvt_f32_bf8(w, 3);
+}
+
 // 8 codes of 4 bits as an operand of 8 halves, times `scale`, a power of two.
 __device__ __forceinline__ f16x8 halves4(uint32_t w, float scale) {
   const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
@@ -302,6 +317,18 @@ __device__ __forceinline__ f16x8 scales4(uint32_t lo, uint32_t hi) {
   const u32x4 w = {__builtin_amdgcn_perm(0u, lo, 0x010c000cu), __builtin_amdgcn_perm(0u, lo, 0x030c020cu),
                    __builtin_amdgcn_perm(0u, hi, 0x010c000cu), __builtin_amdgcn_perm(0u, hi, 0x030c020cu)};
   return __builtin_bit_cast(f16x8, w);
+}
+// Word t of the lanes l, l ^ 16, l ^ 32, l ^ 48 is in lane group t: byte g of each for lane group g, in their order.
+__device__ __forceinline__ uint32_t turn_bytes(uint32_t w, int g) {
+  const auto a = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(a[0], a[0], false, false), hi = __builtin_amdgcn_permlane16_swap(a[1], a[1], false, false);
+  const uint32_t pick = 0x0c0c0400u + 0x0101u * g;
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(hi[1], hi[0], pick), __builtin_amdgcn_perm(lo[1], lo[0], pick), 0x05040100u);
+}
+// What lane LANE of each 16 has, in all of them.
+template <int LANE>
+__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + LANE, 0xf, 0xf, true);
 }
 // Scales of tokens 4 w .. 4 w + 3 of which only the first `seen - 4 w` count.
 __device__ __forceinline__ uint32_t keep_bytes(int left) {

@@ -22,13 +22,18 @@ namespace pp {
 // prompts of two row tiles a CU and more.  Cut / whole, 4 prompts: 256 row tiles 53 / 50, 384 117 / 68, 512 144 / 99,
 // 1024 503 / 333; behind 4000 tokens each 128 115 / 144, 256 193 / 172, 320 246 / 288, 384 301 / 308, 448 363 / 328.
 // What lies behind a prompt only the device knows; whole tiles never lose from 448 on.
+//
+// 4 bits, few rows, to 128 values a head: two workgroups a CU where there are as many row tiles as CUs, so that few are
+// cut into many parts.  One / two, in us: 256 row tiles (128 sequences of 1000-8000, 2 key heads) 45.9 / 43.2, 512 (64 of
+// 500-1000, 8) 33.1 / 30.7; 128 (16 of 8000-16,000, 8) 50.2 / 51.0, 64 (8 of 30-40,000) 63.8 / 64.6, 8 21.9 / 25.8.
 static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
-                          int64_t q_heads) {
+                          int64_t q_heads, bool four) {
   const int64_t group = q_heads / heads, rows = (tokens * group + batch - 1) / batch, cus = device_cu_count();
   AttnPlan P;
   P.rows = rows <= 16 ? 16 : rows <= (D <= 192 ? 64 : 32) ? 32 : rows <= 128 || D > 128 ? 128 : 256;
   const int64_t row_tiles = tokens * group / P.rows + batch + 1;
-  P.shares = ((P.rows <= 32 && D == 64 ? 2 : 1) * cus + heads - 1) / heads;
+  const bool two = P.rows <= 32 && (D == 64 || (four && P.rows == 16 && D == 128 && batch * heads >= cus));
+  P.shares = ((two ? 2 : 1) * cus + heads - 1) / heads;
   const int64_t most = row_tiles * ((width * block + 255) / 256 + 1);       // of 4 tiles each
   if (P.shares > most) P.shares = most;
   if (batch > KV_DEAL_BATCH || (P.rows > 32 && tokens * q_heads / P.rows >= 2 * cus)) P.shares = 0;
@@ -45,7 +50,11 @@ using namespace pp;
 static bool attn_sizes(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
                        int64_t q_heads, AttnPlan* P) {
   if (heads <= 0 || D <= 0 || block <= 0 || width <= 0 || batch <= 0 || tokens <= 0 || q_heads < heads) return false;
-  *P = attn_plan(heads, D, block, width, batch, tokens, q_heads);
+  // what either kind of codes needs
+  *P = attn_plan(heads, D, block, width, batch, tokens, q_heads, false);
+  const AttnPlan four = attn_plan(heads, D, block, width, batch, tokens, q_heads, true);
+  P->bytes = P->bytes > four.bytes ? P->bytes : four.bytes;
+  P->counts = P->counts > four.counts ? P->counts : four.counts;
   return true;
 }
 
@@ -79,7 +88,8 @@ extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t 
   if (tokens == 0) return PP_OK;
   PP_REQUIRE(q && out, "pp_kv_attention: null queries or output");
   PP_REQUIRE(aligned(q, 2) && aligned(out, 16), "pp_kv_attention: queries or output are not aligned");
-  const AttnPlan P = attn_plan(A.C.heads, cache->head_dim, A.C.block, table_width, batch, tokens, q_heads);
+  const AttnPlan P = attn_plan(A.C.heads, cache->head_dim, A.C.block, table_width, batch, tokens, q_heads,
+                               cache->codes == PP_KV_E2M1);
   PP_REQUIRE(P.bytes == 0 || (workspace && workspace_size >= P.bytes && aligned(workspace, 16)),
              "pp_kv_attention: workspace of %lld bytes at a 16-byte boundary needed", (long long)P.bytes);
   PP_REQUIRE(P.counts == 0 || (counts && counts_size >= P.counts && aligned(counts, 4)),

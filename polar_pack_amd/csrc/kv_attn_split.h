@@ -36,10 +36,18 @@ namespace pp {
 // two.  64 sequences of 77-8190 with 4 key heads of 192: 80 us (5.2 TB/s); of 256 105 (5.3), where 48-76 bytes a lane
 // spill in tiles of 16 rows and 152-200 in tiles of 32.  V with the streaming cache policy, since a load takes whole lines of it; not K,
 // whose lines two loads share.
+//
+// In 4 bits (PP_KV_E2M1) the codes become halves on their way into the products, K's with their scale, V's times theirs (all
+// exact), and no scale is left for scores or weights.  One tile on its way and two workgroups a CU: converting takes as long
+// as the loads, and a SIMD issues an instruction of one wavefront every 8 clocks, of two every 4 to 5.  64 sequences of
+// 77-8190 tokens and 8 key heads (297 MB) 64 us, 4.6 TB/s, with one workgroup of two tiles a CU 73; loads alone take
+// 62.  4 sequences of 200-262 k and 2 (263 MB) 57 us: there two workgroups a CU would leave twice the parts to join (61).
+// The scaled products that take 4-bit codes as they are were no way: against queries split over three e4m3 terms they are off
+// by 2^-15 of the sum of magnitudes, where float32 sums are by 2^-24.
 template <int CODES, typename IO, int D, int RT, int NP>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(256, D == 64 || (CODES == PP_KV_E2M1 && D * RT == 128) ? 2 : 1) void kv_attn_split_kernel(const AttnArgs A) {
   constexpr bool FOUR = CODES == PP_KV_E2M1;
-  constexpr int DT = D / 16, R = 16 * RT, BUF = D * RT <= 256 ? 2 : 1;
+  constexpr int DT = D / 16, R = 16 * RT, BUF = !FOUR && D * RT <= 256 ? 2 : 1;
   constexpr int EL = FOUR && D % 128 == 0 ? 32 : 16, J = D / (4 * EL), PIECES = EL / 8;   // codes a load of K, loads a row
   typedef std::conditional_t<FOUR && EL == 16, u32x2, u32x4> KWords;
   typedef std::conditional_t<FOUR, u32x2, u32x4> VWords;
@@ -105,8 +113,11 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
   KWords kc[BUF][4][J];
   VWords vc[BUF][DT];
   float ks[BUF], vs[BUF];
-  uint32_t k4[BUF][4][J];                // 4 bits: the scales
-  u32x4 v4[BUF][D / 32];
+  // 4 bits: the scales.  Every lane loads one word, not the bytes and words that it wants: with 32 codes a load of K those of a
+  // token's groups, which then change places with the lanes of the same row; of V those of four tokens and a group, which the
+  // lane's 16 neighbours then read from it.  6 loads a tile less (64 sequences of 77-8190 tokens 75.2 -> 73.2 us).
+  constexpr int KL = EL == 32 ? J : 4 * J, VL = (D / 32 * 4 + 15) / 16;
+  uint32_t k4[BUF][KL], v4[BUF][VL];
   int ok[BUF];
   int64_t vat[BUF];
   auto load_k = [&](auto buf, int tile, int step) {
@@ -125,14 +136,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
     if constexpr (FOUR) {
       const int64_t row = hk * bs + (there ? tok + (m16 & 3) : 0);
       const uint8_t* at = C.k + row * (D / 2) + EL / 2 * g;
-      const uint8_t* sat = scales_k(C) + row * (D / 32) + EL * g / 32;
+      const uint8_t* sat = scales_k(C) + row * (D / 32) + (EL == 32 ? 4 * g * (D / 32) : EL * g / 32);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           kc[I][t][j] = *reinterpret_cast<const KWords*>(at + 4 * t * (D / 2) + 2 * EL * j);
-          k4[I][t][j] = sat[4 * t * (D / 32) + EL / 8 * j];
+          if constexpr (EL == 16) k4[I][4 * j + t] = sat[4 * t * (D / 32) + EL / 8 * j];
         }
+      if constexpr (EL == 32) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) k4[I][j] = *reinterpret_cast<const uint32_t*>(sat + 4 * j);      // of token t = g
+      }
       vat[I] = ph * (bs * D) + (there ? (tile * 64 + 16 * g) & (bs - 1) : 0);      // as codes of a byte
       return;
     }
@@ -154,7 +169,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
       const int64_t page = vat[I] & ~(int64_t)(bs - 1);        // page and head * bs * D
       const uint8_t* at = scales_v(C) + (page >> 5) + (vat[I] - page);
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) v4[I][d] = *reinterpret_cast<const u32x4*>(at + d * bs);
+      for (int i = 0; i < VL; ++i)
+        v4[I][i] = *reinterpret_cast<const uint32_t*>(at + min(4 * i + (m16 >> 2), D / 32 - 1) * bs + 4 * (m16 & 3));
       return;
     }
 #pragma unroll
@@ -188,6 +204,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
   auto work = [&](auto buf) {
     constexpr int I = decltype(buf)::value;
     f32x4 s[RT][4];
+    if constexpr (FOUR && EL == 32) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) k4[I][j] = turn_bytes(k4[I][j], g);
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -195,7 +215,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         if constexpr (FOUR) {
-          const float ks4 = __builtin_amdgcn_cvt_f32_bf8(k4[I][t][j], 0);
+          const float ks4 = EL == 16 ? __builtin_amdgcn_cvt_f32_bf8(k4[I][EL == 16 ? 4 * j + t : 0], 0) : bf8_byte(k4[I][j], t);
 #pragma unroll
           for (int w = 0; w < PIECES; ++w) {
             const f16x8 ka = halves4(kc[I][t][j][w], ks4);
@@ -270,13 +290,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
     if (CODES != PP_KV_INT8) {                   // past the length codes may be NaN, and scales of 4 bits
       const int seen = okv ? T.lim - t0 : 0;
       if (__any(seen < 16)) {
+        if constexpr (FOUR) {
+          const uint32_t keep = keep_bytes(seen - 4 * (m16 & 3));
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t keep = keep_bytes(seen - 4 * w);
-          if constexpr (FOUR) {
+          for (int i = 0; i < VL; ++i) v4[I][i] &= keep;
+        } else {
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) v4[I][d][w] &= keep;
-          } else {
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t keep = keep_bytes(seen - 4 * w);
 #pragma unroll
             for (int d = 0; d < DT; ++d) vc[I][d][w] &= keep;
           }
@@ -284,13 +305,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
       }
     }
     f16x8 sa, sb;                                // of the tokens' scales
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
+    each<DT>([&](auto dt) {
+      constexpr int d = decltype(dt)::value;
       f16x8 va, vb;
       if constexpr (FOUR) {
-        if (d % 2 == 0) {
-          sa = scales4(v4[I][d / 2][0], v4[I][d / 2][1]);
-          sb = scales4(v4[I][d / 2][2], v4[I][d / 2][3]);
+        if constexpr (d % 2 == 0) {
+          constexpr int at = 2 * d % 16;
+          const uint32_t w = v4[I][d / 8];
+          sa = scales4(row_bcast<at>(w), row_bcast<at + 1>(w));
+          sb = scales4(row_bcast<at + 2>(w), row_bcast<at + 3>(w));
         }
         va = halves4(vc[I][d][0], 1.f) * sa;
         vb = halves4(vc[I][d][1], 1.f) * sb;
@@ -302,7 +325,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void kv_attn_split_kernel(con
         o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[x][0], o[x][d], 0, 0, 0);
         o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, p[x][1], o[x][d], 0, 0, 0);
       }
-    }
+    });
     load_v(buf);
     tile += 4;
     ++step;

@@ -16,6 +16,17 @@ class Verified(NamedTuple):
     accepted: torch.Tensor
 
 
+def _rows(x):
+    """A (B, rows, V) tensor whose rows lie one value after another and hold them as they are, and its strides."""
+    if x.is_neg():                                   # memory that holds the values negated
+        x = x.resolve_neg()
+    sb, sr, sv = x.stride()
+    if sv != 1 and x.shape[2] > 1:
+        x = x.contiguous()
+        sb, sr, _ = x.stride()
+    return x, sb, sr
+
+
 def verify_drafts(target, draft, tokens, uniforms, counts=None):
     """Check drafted ``tokens`` (B, n) int64 against the target's probabilities, with given random numbers.
 
@@ -48,16 +59,18 @@ def verify_drafts(target, draft, tokens, uniforms, counts=None):
     if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,)):
         raise TypeError(f"counts must be int32 ({B},)")
     dev = target.device
-    if dev.type != "cuda" or any(t is not None and t.device != dev for t in (draft, tokens, uniforms, counts)):
+    if dev.type != "cuda" or tokens.device != dev or uniforms.device != dev or \
+            draft is not None and draft.device != dev or counts is not None and counts.device != dev:
         raise ValueError("all operands must be on one ROCm device (tensor.device.type == 'cuda')")
-    target, draft, uniforms = (t.resolve_neg() if t is not None and t.is_neg() else t for t in (target, draft, uniforms))
-    if target.stride(2) != 1 and V > 1:
-        target = target.contiguous()
-    if draft is not None and draft.stride(2) != 1 and V > 1:
-        draft = draft.contiguous()
-    if n and tokens.stride(1) != 1 and n > 1:
+    target, p_sb, p_sr = _rows(target)
+    q_sb = q_sr = 0
+    if draft is not None:
+        draft, q_sb, q_sr = _rows(draft)
+    if uniforms.is_neg():
+        uniforms = uniforms.resolve_neg()
+    if n > 1 and tokens.stride(1) != 1:
         tokens = tokens.contiguous()
-    if uniforms.stride(1) != 1 and n > 0:
+    if n > 0 and uniforms.stride(1) != 1:
         uniforms = uniforms.contiguous()
     if counts is not None and not counts.is_contiguous():
         counts = counts.contiguous()
@@ -67,9 +80,8 @@ def verify_drafts(target, draft, tokens, uniforms, counts=None):
         size = nat.sized("pp_verify_drafts_workspace_size", dev.index, B, V)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         done, key = nat.zero_workspace(dev, 4 * B)
-        rc = nat.lib().pp_verify_drafts(target.data_ptr(), target.stride(0), target.stride(1),
-                                        draft.data_ptr() if draft is not None and n else None,
-                                        draft.stride(0) if draft is not None else 0, draft.stride(1) if draft is not None else 0,
+        rc = nat.lib().pp_verify_drafts(target.data_ptr(), p_sb, p_sr,
+                                        draft.data_ptr() if draft is not None and n else None, q_sb, q_sr,
                                         _PROBABILITIES[target.dtype], B, n, V, tokens.data_ptr() if n else None,
                                         tokens.stride(0), uniforms.data_ptr(), uniforms.stride(0),
                                         counts.data_ptr() if counts is not None else None, out.data_ptr(),
