@@ -169,6 +169,21 @@ __device__ __forceinline__ void append_page(const KvCache& C, const Piece& P, in
   }
 }
 
+// Values `at` .. at + 7 of the rows of a piece's tokens 4 tg .. 4 tg + 3; where one is not of the piece, of its nearest row.
+// No branch lies between the loads, which would make the compiler wait for each.
+__device__ __forceinline__ void load_rows(const Piece& P, const uint16_t* src, int64_t st, int vec, int tg, int at, u32x4* x) {
+  const uint16_t* row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = src + (P.row0 + min(max(4 * tg + i, P.lo), P.hi - 1)) * st + at;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = load8(row[i], true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = load8(row[i], false);
+  }
+}
+
 // The 16-bit values of a piece that thread (tg, dg) holds, zeros where there are none, and the largest word of
 // magnitudes: those of 16-bit values are ordered like their words, NaN last.
 template <int D>
@@ -176,16 +191,16 @@ __device__ __forceinline__ uint32_t load_unit(const Piece& P, const uint16_t* sr
                                               u32x4* x) {
   const int tg = tid / (D / 8), dg = tid % (D / 8);
   u16x2 big = {0, 0};
+  load_rows(P, src, st, vec, tg, 8 * dg, x);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int t = 4 * tg + i;
-    x[i] = u32x4{0, 0, 0, 0};
-    if (mine && t >= P.lo && t < P.hi) x[i] = load8(src + (P.row0 + t) * st + 8 * dg, vec);
+    const bool in = mine && 4 * tg + i >= P.lo && 4 * tg + i < P.hi;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[i][j] = in ? x[i][j] : 0u;
+      big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, x[i][j] & 0x7fff7fffu));
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, x[i][j] & 0x7fff7fffu));
   return max((uint32_t)big[0], (uint32_t)big[1]);
 }
 

@@ -131,9 +131,9 @@ __global__ __launch_bounds__(256, D == 64 || (CODES == PP_KV_E2M1 && D * RT == 1
     const int pk = page_of(step, km), pv = page_of(step, vm);
     const int64_t hk = (int64_t)((there & (pk >= 0)) ? pk : 0) * C.heads + (there ? h : 0);
     const int tok = (tile * 64 + 16 * (m16 >> 2)) & (bs - 1);
-    const int64_t ph = (int64_t)((there & (pv >= 0)) ? pv : 0) * C.heads + (there ? h : 0);
-    ok[I] = pv >= 0;
     if constexpr (FOUR) {
+      const int64_t ph = (int64_t)((there & (pv >= 0)) ? pv : 0) * C.heads + (there ? h : 0);
+      ok[I] = pv >= 0;
       const int64_t row = hk * bs + (there ? tok + (m16 & 3) : 0);
       const uint8_t* at = C.k + row * (D / 2) + EL / 2 * g;
       const uint8_t* sat = scales_k(C) + row * (D / 32) + (EL == 32 ? 4 * g * (D / 32) : EL * g / 32);
@@ -156,6 +156,8 @@ __global__ __launch_bounds__(256, D == 64 || (CODES == PP_KV_E2M1 && D * RT == 1
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int j = 0; j < J; ++j) kc[I][t][j] = *reinterpret_cast<const KWords*>(at + 4 * t * D + 64 * j);
+    ok[I] = pv >= 0;
+    const int64_t ph = (int64_t)((there & (pv >= 0)) ? pv : 0) * C.heads + (there ? h : 0);
     ks[I] = C.ks[ph];
     vs[I] = C.vs[ph];
     vat[I] = ph * (bs * D) + (there ? ((tile * 64 + 16 * g) & (bs - 1)) + m16 * bs : 0);
@@ -304,28 +306,35 @@ __global__ __launch_bounds__(256, D == 64 || (CODES == PP_KV_E2M1 && D * RT == 1
         }
       }
     }
-    f16x8 sa, sb;                                // of the tokens' scales
-    each<DT>([&](auto dt) {
-      constexpr int d = decltype(dt)::value;
-      f16x8 va, vb;
-      if constexpr (FOUR) {
+    if constexpr (FOUR) {
+      f16x8 sa, sb;                              // of the tokens' scales
+      each<DT>([&](auto dt) {
+        constexpr int d = decltype(dt)::value;
         if constexpr (d % 2 == 0) {
           constexpr int at = 2 * d % 16;
           const uint32_t w = v4[I][d / 8];
           sa = scales4(row_bcast<at>(w), row_bcast<at + 1>(w));
           sb = scales4(row_bcast<at + 2>(w), row_bcast<at + 3>(w));
         }
-        va = halves4(vc[I][d][0], 1.f) * sa;
-        vb = halves4(vc[I][d][1], 1.f) * sb;
-      } else {
-        to_halves<CODES>(vc[I][d], va, vb);
-      }
+        const f16x8 va = halves4(vc[I][d][0], 1.f) * sa, vb = halves4(vc[I][d][1], 1.f) * sb;
 #pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[x][0], o[x][d], 0, 0, 0);
-        o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, p[x][1], o[x][d], 0, 0, 0);
+        for (int x = 0; x < RT; ++x) {
+          o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[x][0], o[x][d], 0, 0, 0);
+          o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, p[x][1], o[x][d], 0, 0, 0);
+        }
+      });
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        f16x8 va, vb;
+        to_halves<CODES>(vc[I][d], va, vb);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+          o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[x][0], o[x][d], 0, 0, 0);
+          o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, p[x][1], o[x][d], 0, 0, 0);
+        }
       }
-    });
+    }
     load_v(buf);
     tile += 4;
     ++step;

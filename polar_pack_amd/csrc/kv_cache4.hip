@@ -66,7 +66,7 @@ __global__ __launch_bounds__(TURN ? 512 : 256, TURN ? 3 : 4) void kv_append4_ker
   __syncthreads();
   uint32_t& flags = bad[sub];
   u32x4 xv[4];
-  load_unit<D>(P, A.x[1] + (int64_t)head * A.sh[1], A.st[1], A.vec, tid, mine, xv);
+  load_unit<D>(P, A.x[1] + (int64_t)min(head, C.heads - 1) * A.sh[1], A.st[1], A.vec, tid, mine, xv);
   uint32_t kw[4], kb[4], vb = 0, lost = 0;
   auto code_keys = [&](int i, const real* x) {
     float f[8];
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(TURN ? 512 : 256, TURN ? 3 : 4) void kv_append4_ker
     kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[4], f[5], s, 2);
     kw[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(kw[i], f[6], f[7], s, 3);
   };
-  const uint16_t* const keys = A.x[0] + (int64_t)head * A.sh[0];
+  const uint16_t* const keys = A.x[0] + (int64_t)min(head, C.heads - 1) * A.sh[0];
   if constexpr (TURN) {
     load_turned<IO, real, D>(X.R, P, keys, A.st[0], A.vec, tid, mine, tab, code_keys);
   } else {

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(D < 128 ? 512 : 4 * D, 4) void kv_rotate_append_ker
   extern __shared__ __align__(16) uint32_t lds[];      // of keys the table, of values the codes
   const bool active = head < C.heads, mine = active && tid < (C.block / 4) * (D / 8);
   uint32_t* const red = maxima[sub];
-  const uint16_t* src = A.x[isv] + (int64_t)head * A.sh[isv];
+  const uint16_t* src = A.x[isv] + (int64_t)min(head, C.heads - 1) * A.sh[isv];
   if (isv) {
     u32x4 x[4];
     const uint32_t top = load_unit<D>(P, src, A.st[1], A.vec, tid, mine, x);

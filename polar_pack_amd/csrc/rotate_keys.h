@@ -37,15 +37,8 @@ __device__ __forceinline__ void load_turned(const Rot& R, const Piece& P, const 
   const int other = R.neighbours || !turned ? dg : low ? dg + h8 : dg - h8;
   const int f0 = R.neighbours ? 4 * dg : low ? 8 * dg : 8 * (dg - h8);
   u32x4 x[4], y[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 4 * tg + i;
-    x[i] = y[i] = u32x4{0, 0, 0, 0};
-    if (!mine || t < P.lo || t >= P.hi) continue;
-    const uint16_t* row = src + (P.row0 + t) * st;
-    x[i] = load8(row + 8 * dg, vec);
-    y[i] = load8(row + 8 * other, vec);
-  }
+  load_rows(P, src, st, vec, tg, 8 * dg, x);
+  load_rows(P, src, st, vec, tg, 8 * other, y);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * tg + i;
@@ -54,7 +47,8 @@ __device__ __forceinline__ void load_turned(const Rot& R, const Piece& P, const 
     T v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (T)half_of<IO>(x[i], j);
-    if (turned && mine && t >= P.lo && t < P.hi) {
+    const bool in = mine && t >= P.lo && t < P.hi;
+    if (turned && in) {
       const Trig<T>* const row = tab + (t - P.lo) * rot_stride(R);
       auto trig = [&](int f) { return row[rot_place(R, f)]; };
       if (R.neighbours) {
@@ -73,6 +67,10 @@ __device__ __forceinline__ void load_turned(const Rot& R, const Piece& P, const 
           v[j] = v[j] * w.c + (low ? -b : b);
         }
       }
+    }
+    if (!in) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0;
     }
     use(i, v);
     __builtin_amdgcn_sched_barrier(0);
