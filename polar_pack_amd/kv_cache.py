@@ -142,8 +142,9 @@ def _call(cache, block_table, lengths, cu, tokens):
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError("block_table must be int32 (B, width) and lengths int32 (B,)")
     B, width = block_table.shape
+    ld, step = block_table.stride()
     dev = cache.device
-    if lengths.shape != (B,) or lengths.stride(0) != 1 and B > 1 or block_table.stride(1) != 1 and width > 1:
+    if lengths.shape != (B,) or B > 1 and lengths.stride(0) != 1 or step != 1 and width > 1:
         raise ValueError("lengths must be a contiguous (B,) tensor and block_table's rows contiguous")
     if block_table.device != dev or lengths.device != dev:
         raise ValueError("all operands must be on the cache's device")
@@ -152,25 +153,39 @@ def _call(cache, block_table, lengths, cu, tokens):
     if cu is None:
         if tokens != B:
             raise ValueError(f"{tokens} tokens for {B} sequences: cu must say which are whose")
-        return block_table.data_ptr(), block_table.stride(0), width, lengths.data_ptr(), None, B
+        return block_table.data_ptr(), ld, width, lengths.data_ptr(), None, B
     if cu.dtype != torch.int32 or cu.shape != (B + 1,) or not cu.is_contiguous():
         raise TypeError("cu must be a contiguous int32 (B + 1,) tensor")
     if cu.device != dev:
         raise ValueError("all operands must be on the cache's device")
-    return block_table.data_ptr(), block_table.stride(0), width, lengths.data_ptr(), cu.data_ptr(), B
+    return block_table.data_ptr(), ld, width, lengths.data_ptr(), cu.data_ptr(), B
 
 
 def _values(cache, x, name, heads):
-    """A (tokens, heads, D) tensor of 16-bit values with a contiguous last dimension."""
+    """A (tokens, heads, D) tensor of 16-bit values with a contiguous last dimension, and its address and strides."""
     if x.dim() != 3 or x.dtype not in _VALUES:
         raise TypeError(f"{name} must be float16 or bfloat16 (tokens, heads, D)")
-    if x.shape[2] != cache.head_dim or heads is not None and x.shape[1] != heads:
+    shape = x.shape
+    if shape[2] != cache.head_dim or heads is not None and shape[1] != heads:
         raise ValueError(f"{name} must be (tokens, {heads if heads else 'heads'}, {cache.head_dim})")
     if x.device != cache.device:
         raise ValueError("all operands must be on the cache's device")
     if x.is_neg():                                   # memory that holds the values negated
         x = x.resolve_neg()
-    return x if x.stride(2) == 1 else x.contiguous()
+    st, sh, sd = x.stride()
+    if sd != 1:
+        x = x.contiguous()
+        st, sh, _ = x.stride()
+    return x, (x.data_ptr(), st, sh)
+
+
+def _keys_values(cache, k, v):
+    """(k, v, type, addresses and strides for the C entries), checked."""
+    k, at_k = _values(cache, k, "k", cache.heads)
+    v, at_v = _values(cache, v, "v", cache.heads)
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must have one shape and type")
+    return k, v, _VALUES[k.dtype], at_k + at_v
 
 
 def kv_append(cache, k, v, block_table, lengths, cu=None):
@@ -196,16 +211,11 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
     token NaN for every row that sees it, and where it is read.
     """
     _check_cache(cache)
-    k = _values(cache, k, "k", cache.heads)
-    v = _values(cache, v, "v", cache.heads)
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("k and v must have one shape and type")
+    k, v, dtype, at = _keys_values(cache, k, v)          # k and v: what holds the memory until the launch is queued
     n = k.shape[0]
     call = _call(cache, block_table, lengths, cu, n)
     with nat.on_device(cache.device):
-        nat.check(nat.lib().pp_kv_append(cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                         v.stride(0), v.stride(1), _VALUES[k.dtype], n, *call,
-                                         nat.raw_stream(cache.device)), "pp_kv_append")
+        nat.check(nat.lib().pp_kv_append(cache._ref, *at, dtype, n, *call, nat.raw_stream(cache.device)), "pp_kv_append")
 
 
 def kv_rotate_append(cache, q, k, v, rotary, block_table, lengths, cu=None, *, positions=None):
@@ -220,28 +230,24 @@ def kv_rotate_append(cache, q, k, v, rotary, block_table, lengths, cu=None, *, p
     """
     _check_cache(cache)
     dev, D = cache.device, cache.head_dim
-    k = _values(cache, k, "k", cache.heads)
-    v = _values(cache, v, "v", cache.heads)
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("k and v must have one shape and type")
+    k, v, dtype, at_kv = _keys_values(cache, k, v)
     n = k.shape[0]
+    queries = (None, 0, 0, 0)
     if q is not None:
-        q = _values(cache, q, "q", None)
+        q, at_q = _values(cache, q, "q", None)
         if q.shape[0] != n or q.dtype != k.dtype:
             raise ValueError("q must have k's tokens and type")
+        queries = at_q + (q.shape[1],)
     _check_rotary(rotary, D, dev)
     at = (None, 0, nat.PP_POS_I32)
     if positions is not None:
         positions, at = _positions(rotary, positions, n, dev)
     call = _call(cache, block_table, lengths, cu, n)
     with nat.on_device(dev):
-        queries, out = (None, 0, 0, 0, None), None
-        if q is not None:
-            out = torch.empty((n, q.shape[1], D), dtype=q.dtype, device=dev)
-            queries = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], out.data_ptr())
-        nat.check(nat.lib().pp_kv_rotate_append(cache._ref, *queries, k.data_ptr(), k.stride(0), k.stride(1),
-                                                v.data_ptr(), v.stride(0), v.stride(1), _VALUES[k.dtype], n,
-                                                rotary._ref, *at, *call, nat.raw_stream(dev)), "pp_kv_rotate_append")
+        out = torch.empty((n, q.shape[1], D), dtype=q.dtype, device=dev) if q is not None else None
+        nat.check(nat.lib().pp_kv_rotate_append(cache._ref, *queries, out.data_ptr() if out is not None else None, *at_kv,
+                                                dtype, n, rotary._ref, *at, *call, nat.raw_stream(dev)),
+                  "pp_kv_rotate_append")
     return out
 
 
@@ -280,7 +286,7 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
     q_heads) natural logarithms of the sums, by which attention over several caches is joined.
     """
     _check_cache(cache)
-    q = _values(cache, q, "q", None)
+    q, at = _values(cache, q, "q", None)
     n, heads = q.shape[0], q.shape[1]
     if heads == 0 or heads % cache.heads:
         raise ValueError(f"{heads} query heads over {cache.heads} heads")
@@ -297,7 +303,7 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
         n_counts = nat.sized("pp_kv_attention_counts_size", *shape)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         counts, key = nat.zero_workspace(dev, n_counts)
-        rc = nat.lib().pp_kv_attention(cache._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _VALUES[q.dtype], n,
+        rc = nat.lib().pp_kv_attention(cache._ref, *at, heads, _VALUES[q.dtype], n,
                                        *call, int(causal), int(window), scale, out.data_ptr(),
                                        lse.data_ptr() if return_lse else None, ws.data_ptr() if size else None, size,
                                        counts.data_ptr() if n_counts else None, n_counts, nat.raw_stream(dev))

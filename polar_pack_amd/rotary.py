@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from fractions import Fraction
 
 import torch
 
@@ -20,8 +19,16 @@ HEAD_DIM_MAX = 512
 _ROWS = {torch.float16: nat.PP_F16, torch.bfloat16: nat.PP_BF16, torch.float32: nat.PP_F32}
 _POSITIONS = {torch.int32: nat.PP_POS_I32, torch.int64: nat.PP_POS_I64}
 _PAIRS = {"halves": nat.PP_PAIRS_HALVES, "neighbours": nat.PP_PAIRS_NEIGHBOURS}
-# 1 / (2 pi) to 2^-124: a frequency's share of a turn is wanted to 2^-64
-_TURN = Fraction(0x28BE60DB9391054A7F09D5F47D4D377, 1 << 124)
+# 2^124 / (2 pi)
+_TURN = 0x28BE60DB9391054A7F09D5F47D4D377
+
+
+def _turn(freq):
+    """The fraction of a turn that ``freq`` radians are, times 2^64 and rounded, as a signed 64-bit number."""
+    n, d = freq.as_integer_ratio()                   # d is a power of two
+    shift = 60 + d.bit_length() - 1
+    t = ((n * _TURN + (1 << (shift - 1))) >> shift) & ((1 << 64) - 1)
+    return t - (1 << 64) if t >= 1 << 63 else t
 
 
 class Rotary:
@@ -77,8 +84,7 @@ class Rotary:
         if device.type != "cuda":
             raise ValueError("a Rotary lives on a ROCm device (device.type == 'cuda')")
         self.head_dim, self.rotary_dim, self.pairs, self.scaling = head_dim, rotary_dim, pairs, float(scaling)
-        turns = [round(Fraction(f) * _TURN * (1 << 64)) % (1 << 64) for f in freq]
-        turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64)
+        turns = torch.tensor([_turn(f) for f in freq], dtype=torch.int64)
         self._turns = turns.to(device)
         self._axes = None if self.n_axes == 1 else torch.tensor(axes, dtype=torch.uint8).to(device)
         self.device = self._turns.device
@@ -137,12 +143,15 @@ def rotate(x, rotary, positions, *, out=None):
             raise ValueError("out's rows must not overlap")
     if x.is_neg():                                   # memory that holds the values negated
         x = x.resolve_neg()
-    if x.stride(2) != 1:
+    st, sh, sd = x.stride()
+    if sd != 1:
         x = x.contiguous()
+        st, sh, _ = x.stride()
     with nat.on_device(dev):
         if out is None:
-            out = torch.empty((tokens, heads, D), dtype=x.dtype, device=dev)
-        nat.check(nat.lib().pp_rotate(x.data_ptr(), x.stride(0), x.stride(1), _ROWS[x.dtype], tokens, heads, D,
-                                      rotary._ref, *at, out.data_ptr(), out.stride(0), out.stride(1),
-                                      nat.raw_stream(dev)), "pp_rotate")
+            out, o_st, o_sh = torch.empty((tokens, heads, D), dtype=x.dtype, device=dev), heads * D, D
+        else:
+            o_st, o_sh, _ = out.stride()
+        nat.check(nat.lib().pp_rotate(x.data_ptr(), st, sh, _ROWS[x.dtype], tokens, heads, D, rotary._ref, *at,
+                                      out.data_ptr(), o_st, o_sh, nat.raw_stream(dev)), "pp_rotate")
     return out
