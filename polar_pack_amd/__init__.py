@@ -9,8 +9,10 @@ Modules mirror the reference's operator files:
 
 and beside them, for the rest of a decode step:
 
-* :mod:`polar_pack_amd.kv_cache`      -- 8-bit paged key/value cache and its attention
+* :mod:`polar_pack_amd.rotary`        -- rotary positions, of one axis or several
+* :mod:`polar_pack_amd.kv_cache`      -- paged key/value cache in 8 or 4 bits and its attention
 * :mod:`polar_pack_amd.logprobs`      -- log probabilities, entropy, alternatives
+* :mod:`polar_pack_amd.drafts`        -- drafted tokens against the target's probabilities
 
 All compute runs in the HIP library ``lib/libpolar_pack.so`` (C ABI in
 include/polar_pack.h); there is no CPU or eager fallback.
