@@ -26,7 +26,7 @@ def test_steps_do_what_the_definition_says():
     for i in range(6):
         before = models.size.clone()
         u = torch.rand(ex.MODELS, models.drafts + 1, generator=g)
-        if i % 2:
+        if i % 2 == 0:                                       # at first, while the text repeats itself
             u[:, 1:-1] = 0                                    # what has a probability at all is kept
             u[::2, 0] = 0
         target, tokens, counts, r = models.step(u.cuda())
@@ -49,7 +49,7 @@ def test_drafts_that_were_refused_leave_nothing_behind():
     models, g = start(), torch.Generator().manual_seed(3)
     for i in range(5):
         u = torch.rand(ex.MODELS, models.drafts + 1, generator=g)
-        if i % 2:
+        if i % 2 == 0:                                       # at first, while the text repeats itself
             u[:, :2] = 0
         models.step(u.cuda())
     last = models.text.gather(1, models.size[:, None] - 1)
