@@ -75,8 +75,8 @@ def verify_drafts(target, draft, tokens, uniforms, counts=None):
     if counts is not None and not counts.is_contiguous():
         counts = counts.contiguous()
     with nat.on_device(dev):
-        out = torch.empty((B, n + 1), dtype=torch.int64, device=dev)
-        accepted = torch.empty((B,), dtype=torch.int64, device=dev)
+        out = torch.empty(B, n + 1, dtype=torch.int64, device=dev)
+        accepted = torch.empty(B, dtype=torch.int64, device=dev)
         size = nat.sized("pp_verify_drafts_workspace_size", dev.index, B, V)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         done, key = nat.zero_workspace(dev, 4 * B)

@@ -244,7 +244,7 @@ def kv_rotate_append(cache, q, k, v, rotary, block_table, lengths, cu=None, *, p
         positions, at = _positions(rotary, positions, n, dev)
     call = _call(cache, block_table, lengths, cu, n)
     with nat.on_device(dev):
-        out = torch.empty((n, q.shape[1], D), dtype=q.dtype, device=dev) if q is not None else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if q is not None else None
         nat.check(nat.lib().pp_kv_rotate_append(cache._ref, *queries, out.data_ptr() if out is not None else None, *at_kv,
                                                 dtype, n, rotary._ref, *at, *call, nat.raw_stream(dev)),
                   "pp_kv_rotate_append")
@@ -264,7 +264,7 @@ def kv_read(cache, block_table, lengths, cu=None, *, total=None, dtype=torch.flo
         total = block_table.shape[0]
     call = _call(cache, block_table, lengths, cu, total)
     with nat.on_device(cache.device):
-        out = torch.empty((2, total, cache.heads, cache.head_dim), dtype=dtype, device=cache.device)
+        out = torch.empty(2, total, cache.heads, cache.head_dim, dtype=dtype, device=cache.device)
         k, v = out.unbind(0)
         nat.check(nat.lib().pp_kv_read(cache._ref, *call, total, _READS[dtype], k.data_ptr(), v.data_ptr(),
                                        nat.raw_stream(cache.device)), "pp_kv_read")
@@ -296,8 +296,8 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
     dev = cache.device
     with nat.on_device(dev):
-        out = torch.empty((n, heads, cache.head_dim), dtype=q.dtype, device=dev)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = torch.empty(n, heads, dtype=torch.float32, device=dev) if return_lse else None
         shape = (dev.index, cache.heads, cache.head_dim, cache.block, call[2], call[5], n, heads)
         size = nat.sized("pp_kv_attention_workspace_size", *shape)
         n_counts = nat.sized("pp_kv_attention_counts_size", *shape)

@@ -149,7 +149,7 @@ def rotate(x, rotary, positions, *, out=None):
         st, sh, _ = x.stride()
     with nat.on_device(dev):
         if out is None:
-            out, o_st, o_sh = torch.empty((tokens, heads, D), dtype=x.dtype, device=dev), heads * D, D
+            out, o_st, o_sh = torch.empty_like(x, memory_format=torch.contiguous_format), heads * D, D
         else:
             o_st, o_sh, _ = out.stride()
         nat.check(nat.lib().pp_rotate(x.data_ptr(), st, sh, _ROWS[x.dtype], tokens, heads, D, rotary._ref, *at,
