@@ -151,6 +151,12 @@ struct Deal {
   int into;           // tile of the row tile that `at` is, KV_TURN the first that holds keys
 };
 
+// a / b for a >= 0, b > 0: a call has seldom 2^32 tiles, and a 64-bit division is some 150 instructions, which few wavefronts
+// take half a microsecond for.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (uint64_t)(a | b) >> 32 == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // What sequence b's row tiles have to read, and its rows.
 __device__ __forceinline__ int kv_sequence(const AttnArgs& A, int b, RowTile& T, int& first, int& tiles) {
   const KvSeqs& S = A.S;
@@ -206,7 +212,7 @@ __device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, De
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) all += sums[w];
   for (int w = 0; w < wave; ++w) upto += sums[w];
-  const int64_t share = (all + A.shares - 1) / A.shares;
+  const int64_t share = quotient(all + A.shares - 1, A.shares);
   U.share = (int)(share < 4 ? 4 : (share + 3) / 4 * 4);        // 4 wavefronts a workgroup
   U.at = (int64_t)blockIdx.x * U.share;
   U.end = U.at + U.share < all ? U.at + U.share : all;
@@ -235,7 +241,7 @@ __device__ __forceinline__ bool kv_deal(const AttnArgs& A, int R, RowTile& T, De
   U.first = uniform(found[5]);
   U.tiles = uniform(found[6]);
   const int64_t t = uniform64(from);
-  const int row_tile = (int)(t / (U.tiles + KV_TURN));
+  const int row_tile = (int)quotient(t, U.tiles + KV_TURN);
   T.r0 = row_tile * R;
   U.into = (int)(t - (int64_t)row_tile * (U.tiles + KV_TURN));
   return true;

@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256, D == 64 || (CODES == PP_KV_E2M1 && D * RT == 1
     const int t0 = max(U.into - KV_TURN, 0), t1 = U.into + take - KV_TURN;
     U.at += take;
     if (t1 <= 0) return;                                       // the share ends before them
-    owner = (int)(begin / U.share);
-    runs = (int)((begin + U.tiles - 1) / U.share) - owner + 1;
+    owner = (int)quotient(begin, U.share);
+    runs = (int)quotient(begin + U.tiles - 1, U.share) - owner + 1;
     run = blockIdx.x - owner;
     kv_tile_range(A, R, T);
     a = max(U.first + t0, T.lo >> 6);
