@@ -92,8 +92,8 @@ class KVCache4:
     earlier one in its low half: ``k`` uint8 (pages, heads, block, D / 2), ``v`` uint8 (pages, heads, D, block / 2).
     Every 32 values of a token and head share a scale, a power of two from 2**-14 to 2**13 as float8_e5m2:
     ``k_scale`` (pages, heads, block, D / 32), ``v_scale`` (pages, heads, D / 32, block).  4.25 bits a value; a
-    token's codes depend on no other token.  A NaN in a token's ``k_scale`` makes the token NaN for every row that
-    sees it; scales of tokens before a sequence's length are otherwise as :func:`kv_append` writes them.  What lies past
+    token's codes depend on no other token.  NaN as each of a token's ``k_scale`` makes the token NaN for every row
+    that sees it; scales of tokens before a sequence's length are otherwise as :func:`kv_append` writes them.  What lies past
     the lengths may hold anything.
     :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.
     """
@@ -204,7 +204,7 @@ def kv_append(cache, k, v, block_table, lengths, cu=None):
 
     In 4 bits, for every 32 values of a token and head::
 
-        scale = the smallest power of two in [2**-14, 2**13] with max|x| <= 7 * scale
+        scale = the smallest power of two in [2**-14, 2**13] with max|x| <= 7 * scale (2**13 where none is)
         code  = the nearest to x / scale           ties to even, held to +-6
 
     Both are exact functions of the values.  A value that is not finite, of the key or the value, makes the

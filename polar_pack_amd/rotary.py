@@ -139,8 +139,11 @@ def rotate(x, rotary, positions, *, out=None):
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and not x.is_neg()
         if not same and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise ValueError("out must be x itself or share no memory with it")
-        if out.numel() and any(out.stride(i) == 0 and out.shape[i] > 1 for i in (0, 1)):
-            raise ValueError("out's rows must not overlap")
+        reach = D                                    # of the rows along the nearer stride, then along both
+        for step, rows in sorted((out.stride(i), out.shape[i]) for i in (0, 1) if out.numel() and out.shape[i] > 1):
+            if step < reach:
+                raise ValueError("out's rows must not overlap")
+            reach += step * (rows - 1)
     if x.is_neg():                                   # memory that holds the values negated
         x = x.resolve_neg()
     st, sh, sd = x.stride()

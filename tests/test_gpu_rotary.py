@@ -179,3 +179,18 @@ def test_refusals():
                      (lambda: rotate(x[:, :1], r, pos, out=x[:, 1:]), ValueError)):
         with pytest.raises(exc):
             bad()
+
+
+def test_out_whose_rows_overlap_is_refused():
+    r = Rotary(64)
+    x, pos = torch.randn(3, 2, 64, device=DEV).half(), torch.arange(3, device=DEV)
+    room = torch.zeros(1024, device=DEV, dtype=torch.float16)
+    for strides in ((0, 64, 1), (64, 64, 1), (128, 32, 1), (127, 64, 1), (64, 191, 1)):
+        with pytest.raises(ValueError):
+            rotate(x, r, pos, out=room.as_strided((3, 2, 64), strides))
+    assert not room.any()
+    want = rotate(x, r, pos)
+    for strides in ((128, 64, 1), (64, 192, 1), (300, 70, 1)):
+        assert torch.equal(rotate(x, r, pos, out=room.as_strided((3, 2, 64), strides)), want)
+    one = room.as_strided((1, 2, 64), (0, 64, 1))                  # a stride that nothing steps along
+    assert torch.equal(rotate(x[:1], r, pos[:1], out=one), want[:1])
