@@ -7,7 +7,7 @@
 // between: a step of 4 bits is wide, and a rounding before it would move one value in some 10^7 by a whole step.
 //
 // What bounds it: instructions beside memory.  16 ragged prompts (14,752 tokens), 8 key heads and 32 query heads of 128
-// in bf16, 305 MB: 80 us, 3.8 TB/s with the vector units 49 % busy; the queries' rows alone would take 44, the keys and
+// in bf16, 305 MB: 78 us, 3.9 TB/s with the vector units 49 % busy; the queries' rows alone would take 44, the keys and
 // values alone 31 (not turned 18).  The keys' sines in 64 bits, once for four heads, and their rounding to odd are a third of the
 // instructions.  64 single tokens 7.9 us, latency.  Reading back 17 us (58 MB written, 4.7 TB/s).
 #include "kv_cache4.h"
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(TURN ? 512 : 256, TURN ? 3 : 4) void kv_append4_ker
   typedef std::conditional_t<TURN, double, float> real;
   unsigned index = blockIdx.x;
   if (TURN && !X.roles.appends(blockIdx.x, index)) {
-    rotate_queries<IO>(X.A.S, X.R, X.Q, index);
+    rotate_queries<IO, 2>(X.A.S, X.R, X.Q, index);
     return;
   }
   const AppendArgs& A = X.A;

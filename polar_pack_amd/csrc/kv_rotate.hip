@@ -21,7 +21,7 @@ template <int CODES, typename IO, int D>
 __global__ __launch_bounds__(D < 128 ? 512 : 4 * D, 4) void kv_rotate_append_kernel(const RotateArgs X) {
   unsigned index;
   if (!X.roles.appends(blockIdx.x, index)) {
-    rotate_queries<IO>(X.A.S, X.R, X.Q, index);
+    rotate_queries<IO, 1>(X.A.S, X.R, X.Q, index);
     return;
   }
   const AppendArgs& A = X.A;

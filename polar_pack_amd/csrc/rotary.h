@@ -93,24 +93,31 @@ __device__ __forceinline__ Trig<T> rot_trig(const Rot& R, int f, int64_t positio
   return o;
 }
 
-// 8 consecutive values as floats; `vec`: at a 16-byte boundary.
+// 8 consecutive values as they lie in memory; `vec`: at a 16-byte boundary.
 template <typename IO>
-__device__ __forceinline__ void load_row(const typename IO::raw* p, bool vec, float* x) {
-  if constexpr (sizeof(typename IO::raw) == 4) {
-    if (vec) {
-      const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+struct Row8 {
+  u32x4 w[sizeof(typename IO::raw) / 2];
+  __device__ __forceinline__ void load(const typename IO::raw* p, bool vec) {
+    if constexpr (sizeof(typename IO::raw) == 4) {
+      if (vec) {
+        w[0] = reinterpret_cast<const u32x4*>(p)[0];
+        w[1] = reinterpret_cast<const u32x4*>(p)[1];
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(p[i]);
+      }
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p[i];
+      w[0] = load8(p, vec);
     }
-  } else {
-    const u32x4 w = load8(p, vec);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = IO::get((uint16_t)(w[i / 2] >> (16 * (i & 1))));
   }
-}
+  __device__ __forceinline__ void get(float* x) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(typename IO::raw) == 4) x[i] = __uint_as_float(w[i / 4][i % 4]);
+      else x[i] = IO::get((uint16_t)(w[0][i / 2] >> (16 * (i & 1))));
+    }
+  }
+};
 template <typename IO>
 __device__ __forceinline__ void store_row(typename IO::raw* p, bool vec, const float* x) {
   if (!vec) {
@@ -138,8 +145,11 @@ struct RotRows {
 };
 __host__ __device__ inline int rot_units(int half, int D) { return half / 8 + (D - 2 * half + 15) / 16; }
 
-// `none`: a token of no sequence, whose row is zero.
-template <typename IO>
+// `none`: a token of no sequence, whose row is zero.  AHEAD heads are read before the first of them is written: rows may
+// be turned where they lie, so that no load may pass a store before it.  2 beside an append in 4 bits, whose 108
+// registers leave room for few wavefronts (16 ragged prompts 100.5 -> 98.3 us; 3 98.2); 1 beside one in 8 bits, of 78
+// (4 prompts 26.5 us, with 2 27.3), and where rows are all there is (16,200 tokens 26.8 us, with 2 27.2).
+template <typename IO, int AHEAD>
 __device__ __forceinline__ void rotate_unit(const Rot& R, const RotRows& A, int token, int u, int group, int64_t own,
                                             bool none) {
   typedef typename IO::raw raw;
@@ -177,35 +187,47 @@ __device__ __forceinline__ void rotate_unit(const Rot& R, const RotRows& A, int 
   }
   const bool turned = u < units, pairs = R.neighbours;
 #pragma unroll 2
-  for (int h = h0; h < h1; ++h, x += A.x_sh, o += A.o_sh) {
-    float a[8], b[8];
-    load_row<IO>(x + at0, A.vec, a);
-    load_row<IO>(x + at1, A.vec, b);
-    if (turned) {
-      if (pairs) {
+  for (int h = h0; h < h1; h += AHEAD, x += AHEAD * A.x_sh, o += AHEAD * A.o_sh) {
+    Row8<IO> wa[AHEAD], wb[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = a[2 * i], q = a[2 * i + 1], r = b[2 * i], t = b[2 * i + 1];
-          a[2 * i] = p * w[i].c - q * w[i].s;
-          a[2 * i + 1] = q * w[i].c + p * w[i].s;
-          b[2 * i] = r * w[4 + i].c - t * w[4 + i].s;
-          b[2 * i + 1] = t * w[4 + i].c + r * w[4 + i].s;
-        }
-      } else {
+    for (int k = 0; k < AHEAD; ++k) {
+      const raw* const from = x + min(k, h1 - 1 - h) * A.x_sh;
+      wa[k].load(from + at0, A.vec);
+      wb[k].load(from + at1, A.vec);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = a[i], q = b[i];
-          a[i] = p * w[i].c - q * w[i].s;
-          b[i] = q * w[i].c + p * w[i].s;
+    for (int k = 0; k < AHEAD; ++k) {
+      float a[8], b[8];
+      wa[k].get(a);
+      wb[k].get(b);
+      if (turned) {
+        if (pairs) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = a[2 * i], q = a[2 * i + 1], r = b[2 * i], t = b[2 * i + 1];
+            a[2 * i] = p * w[i].c - q * w[i].s;
+            a[2 * i + 1] = q * w[i].c + p * w[i].s;
+            b[2 * i] = r * w[4 + i].c - t * w[4 + i].s;
+            b[2 * i + 1] = t * w[4 + i].c + r * w[4 + i].s;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p = a[i], q = b[i];
+            a[i] = p * w[i].c - q * w[i].s;
+            b[i] = q * w[i].c + p * w[i].s;
+          }
         }
       }
-    }
-    if (none) {
+      if (none) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+        for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+      }
+      if (h + k < h1) {
+        store_row<IO>(o + k * A.o_sh + at0, A.vec, a);
+        store_row<IO>(o + k * A.o_sh + at1, A.vec, b);
+      }
     }
-    store_row<IO>(o + at0, A.vec, a);
-    store_row<IO>(o + at1, A.vec, b);
   }
 }
 

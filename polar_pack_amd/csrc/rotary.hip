@@ -24,7 +24,7 @@ int rot_check(const pp_rotary* r, const void* positions, int64_t pos_ld, int pos
 template <typename IO>
 __global__ __launch_bounds__(256) void rotate_kernel(const Rot R, const RotRows A) {
   const int token = blockIdx.x * blockDim.y + threadIdx.y;
-  if (token < A.tokens) rotate_unit<IO>(R, A, token, threadIdx.x, blockIdx.y, 0, false);
+  if (token < A.tokens) rotate_unit<IO, 1>(R, A, token, threadIdx.x, blockIdx.y, 0, false);
 }
 
 }  // namespace pp

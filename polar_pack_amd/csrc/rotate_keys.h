@@ -78,7 +78,7 @@ __device__ __forceinline__ void load_turned(const Rot& R, const Piece& P, const 
 }
 
 // Block qb of those that turn the queries' rows; every wavefront of the workgroup calls it.
-template <typename IO>
+template <typename IO, int AHEAD>
 __device__ __forceinline__ void rotate_queries(const KvSeqs& S, const Rot& R, const RotRows& Q, int qb) {
   const int units = rot_units(R.half, Q.D), rows = blockDim.x / units, tiles = (Q.tokens + rows - 1) / rows;
   const int group = qb / tiles, first = (qb - group * tiles) * rows;
@@ -102,7 +102,7 @@ __device__ __forceinline__ void rotate_queries(const KvSeqs& S, const Rot& R, co
     none = b >= S.batch;
     if (real && !none) own = (int64_t)S.lengths[b] - kv_start(S, b + 1) + token;
   }
-  if (real) rotate_unit<IO>(R, Q, token, threadIdx.x - y * units, group, own, none);
+  if (real) rotate_unit<IO, AHEAD>(R, Q, token, threadIdx.x - y * units, group, own, none);
 }
 inline int64_t query_blocks(const Rot& R, const RotRows& Q, unsigned threads) {
   if (Q.x == nullptr || Q.tokens == 0) return 0;
