@@ -121,7 +121,8 @@ def rotate(x, rotary, positions, *, out=None):
 
     ``positions`` int32 or int64: (tokens,) with one axis, (axes, tokens) with several; any numbers, negative ones
     turn back.  Computed in float32 and rounded once to x's type.  ``out`` takes the result: x itself, or a tensor of its
-    shape and type that shares no memory with it; by default a new one.
+    shape and type in a storage of its own (another slice of the tensor that x is a slice of is refused); by default a new
+    one.
     """
     if x.dim() != 3 or x.dtype not in _ROWS:
         raise TypeError("x must be float16, bfloat16 or float32 (tokens, heads, head_dim)")
@@ -138,7 +139,7 @@ def rotate(x, rotary, positions, *, out=None):
             raise ValueError("out must hold its values as they are, a row's one after another")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and not x.is_neg()
         if not same and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
-            raise ValueError("out must be x itself or share no memory with it")
+            raise ValueError("out must be x itself or lie in another storage than x's")
         reach = D                                    # of the rows along the nearer stride, then along both
         for step, rows in sorted((out.stride(i), out.shape[i]) for i in (0, 1) if out.numel() and out.shape[i] > 1):
             if step < reach:
