@@ -122,7 +122,7 @@ def rotate(x, rotary, positions, *, out=None):
     ``positions`` int32 or int64: (tokens,) with one axis, (axes, tokens) with several; any numbers, negative ones
     turn back.  Computed in float32 and rounded once to x's type.  ``out`` takes the result: x itself, or a tensor of its
     shape and type in a storage of its own (another slice of the tensor that x is a slice of is refused); by default a new
-    one.
+    one.  A backward pass that has saved ``out`` raises then, as after torch's own writes in place.
     """
     if x.dim() != 3 or x.dtype not in _ROWS:
         raise TypeError("x must be float16, bfloat16 or float32 (tokens, heads, head_dim)")
@@ -132,7 +132,8 @@ def rotate(x, rotary, positions, *, out=None):
     tokens, heads, D = x.shape
     _check_rotary(rotary, D, dev)
     positions, at = _positions(rotary, positions, tokens, dev)
-    if out is not None:
+    given = out is not None
+    if given:
         if out.shape != x.shape or out.dtype != x.dtype or out.device != dev:
             raise ValueError("out must have x's shape, type and device")
         if out.stride(2) != 1 or out.is_neg():
@@ -158,4 +159,6 @@ def rotate(x, rotary, positions, *, out=None):
             o_st, o_sh, _ = out.stride()
         nat.check(nat.lib().pp_rotate(x.data_ptr(), st, sh, _ROWS[x.dtype], tokens, heads, D, rotary._ref, *at,
                                       out.data_ptr(), o_st, o_sh, nat.raw_stream(dev)), "pp_rotate")
+    if given and not out.is_inference():             # a backward pass that has saved it says so instead of using it
+        torch.autograd.graph.increment_version(out)
     return out
