@@ -130,19 +130,19 @@ __global__ __launch_bounds__(DR_THREADS) void verify_drafts_kernel(const DraftAr
   // every wavefront looks at 64 drafts a round
   const int count = A.counts ? min(max(A.counts[b], 0), A.n) : A.n;
   int accepted = count;
-  for (int i0 = 0; i0 < A.n; i0 += 64) {
+  for (int i0 = 0; i0 < count; i0 += 64) {
     const int i = i0 + lane;
-    bool bad = i >= count;
-    if (i < A.n) {
+    bool bad = false;
+    if (i < count) {
       const int64_t t = tokens[i];
       const bool in = t >= 0 && t < A.V;
       const float pd = in ? dr_clean(IO::get(p[i * A.p_sr + t])) : 0.f;
       const float qd = !q ? 1.f : in ? dr_clean(IO::get(q[i * A.q_sr + t])) : 0.f;
-      bad |= !((double)u[i] * (double)qd < (double)pd);
+      bad = !((double)u[i] * (double)qd < (double)pd);
     }
     const uint64_t mask = __ballot(bad);
     if (mask) {
-      accepted = min(count, i0 + __builtin_ctzll(mask));
+      accepted = i0 + __builtin_ctzll(mask);
       break;
     }
   }
