@@ -62,7 +62,9 @@ class Rotary:
                 raise ValueError("base must be a positive number")
             freq = [float(base) ** (-f / n) for f in range(n)]
         else:
-            freq = [float(f) for f in torch.as_tensor(inv_freq).detach().double().cpu().reshape(-1)]
+            if not torch.is_tensor(inv_freq):        # Python's numbers would become float32
+                inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64)
+            freq = [float(f) for f in inv_freq.detach().double().cpu().reshape(-1)]
         if len(freq) != n or not all(math.isfinite(f) for f in freq):
             raise ValueError(f"inv_freq must hold {n} finite numbers")
         if sections is not None and axes is not None:

@@ -1,4 +1,5 @@
-"""rotate where the first tests of it do not look: tensors that a backward pass has saved."""
+"""rotate where the first tests of it do not look: how frequencies are given, tensors that a backward pass has saved."""
+import numpy as np
 import pytest
 import torch
 
@@ -30,3 +31,21 @@ def test_tensors_without_versions():
     other = torch.empty(3, 2, 64, device=DEV)
     assert torch.equal(rotate(x, r, pos, out=other), want)
     assert torch.equal(rotate(x, r, pos, out=x), want)
+
+
+@pytest.mark.parametrize("kind", [list, tuple, np.array, lambda f: [torch.tensor(x, dtype=torch.float64) for x in f]])
+def test_frequencies_keep_their_bits(kind):
+    """Numbers of 64 bits, however they are given: the default ones, given, turn far positions as the default ones do."""
+    freqs = [10000.0 ** (-f / 32) for f in range(32)]
+    x, pos = torch.randn(4, 2, 64, device=DEV), torch.tensor([1, 4097, 10 ** 6 + 1, -2 ** 40], device=DEV)
+    want = rotate(x, Rotary(64), pos)
+    assert torch.equal(rotate(x, Rotary(64, inv_freq=kind(freqs)), pos), want)
+    assert torch.equal(rotate(x, Rotary(64, inv_freq=torch.tensor(freqs, dtype=torch.float64)), pos), want)
+
+
+def test_frequencies_of_32_bits_are_what_they_are():
+    freqs = torch.tensor([10000.0 ** (-f / 32) for f in range(32)])
+    x, pos = torch.randn(2, 2, 64, device=DEV), torch.tensor([4097, 10 ** 6 + 1], device=DEV)
+    want = rotate(x, Rotary(64, inv_freq=freqs.double()), pos)
+    assert torch.equal(rotate(x, Rotary(64, inv_freq=freqs), pos), want)
+    assert torch.equal(rotate(x, Rotary(64, inv_freq=freqs.numpy()), pos), want)
