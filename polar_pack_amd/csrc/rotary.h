@@ -33,7 +33,8 @@ __device__ __forceinline__ void turn_trig(uint64_t t, Trig<double>& o) {
   const uint32_t k = (uint32_t)((t + (1ull << 61)) >> 62);            // the nearest quarter
   const double x = (double)(int64_t)(t - ((uint64_t)k << 62)) * 3.4061215800865545e-19;   // 2 pi / 2^64
   const double z = x * x;
-  // terms to x^15 and x^14: what is left out is below 2^-52 at pi / 4
+  // terms to x^15 and x^16: what is left out is below 2^-53 at pi / 4 (x^17 / 17! 2^-54, x^18 / 18! 2^-59), and with the
+  // roundings both are within 1.9e-16 (to x^14 the cosine was 1.1e-15 off, and a 4-bit code beside a border the wrong one)
   double s = -7.647163731819816e-13;
   s = fma(s, z, 1.6059043836821613e-10);
   s = fma(s, z, -2.505210838544172e-08);
@@ -42,7 +43,8 @@ __device__ __forceinline__ void turn_trig(uint64_t t, Trig<double>& o) {
   s = fma(s, z, 8.3333333333333332e-03);
   s = fma(s, z, -1.6666666666666666e-01);
   s = fma(s * z, x, x);
-  double c = -1.1470745597729725e-11;
+  double c = 4.779477332387385e-14;
+  c = fma(c, z, -1.1470745597729725e-11);
   c = fma(c, z, 2.08767569878681e-09);
   c = fma(c, z, -2.7557319223985888e-07);
   c = fma(c, z, 2.4801587301587302e-05);
