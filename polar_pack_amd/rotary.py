@@ -19,8 +19,9 @@ HEAD_DIM_MAX = 512
 _ROWS = {torch.float16: nat.PP_F16, torch.bfloat16: nat.PP_BF16, torch.float32: nat.PP_F32}
 _POSITIONS = {torch.int32: nat.PP_POS_I32, torch.int64: nat.PP_POS_I64}
 _PAIRS = {"halves": nat.PP_PAIRS_HALVES, "neighbours": nat.PP_PAIRS_NEIGHBOURS}
-# 2^124 / (2 pi)
+# 2^124 / (2 pi), cut off: a larger frequency's fraction of a turn would be off by more than its rounding to 2^-65
 _TURN = 0x28BE60DB9391054A7F09D5F47D4D377
+_FREQ_MAX = 2.0 ** 58
 
 
 def _turn(freq):
@@ -40,8 +41,8 @@ class Rotary:
 
         a' = scaling * (a cos - b sin)        b' = scaling * (b cos + a sin)
 
-    ``inv_freq`` holds rotary_dim / 2 numbers, by default ``base ** (-2 f / rotary_dim)``; other spacings
-    (stretched contexts) are given that way.  With several axes a token has a position on each:
+    with ``scaling`` held in float32.  ``inv_freq`` holds rotary_dim / 2 numbers up to 2**58, by default
+    ``base ** (-2 f / rotary_dim)``; other spacings (stretched contexts) are given that way.  With several axes a token has a position on each:
     ``sections`` says how many frequencies each axis turns, one axis after another, or ``axes`` names
     the axis of every frequency (in turn, say).  Frequencies are kept as 64-bit fractions of a turn, so angles of
     far positions are as exact as those of near ones; there is no table and no largest position.
@@ -65,8 +66,8 @@ class Rotary:
             if not torch.is_tensor(inv_freq):        # Python's numbers would become float32
                 inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64)
             freq = [float(f) for f in inv_freq.detach().double().cpu().reshape(-1)]
-        if len(freq) != n or not all(math.isfinite(f) for f in freq):
-            raise ValueError(f"inv_freq must hold {n} finite numbers")
+        if len(freq) != n or not all(abs(f) <= _FREQ_MAX for f in freq):
+            raise ValueError(f"inv_freq must hold {n} numbers within +-2**58")
         if sections is not None and axes is not None:
             raise ValueError("give sections or axes, not both")
         if sections is not None:
@@ -80,8 +81,8 @@ class Rotary:
             self.n_axes = max(axes, default=0) + 1
         if len(axes) != n or not 1 <= self.n_axes <= 255 or min(axes) < 0:
             raise ValueError(f"axes must hold {n} numbers from 0 to 254")
-        if not math.isfinite(scaling):
-            raise ValueError("scaling must be finite")
+        if not abs(scaling) <= torch.finfo(torch.float32).max:
+            raise ValueError("scaling must be a float32 number")
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("a Rotary lives on a ROCm device (device.type == 'cuda')")
