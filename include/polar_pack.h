@@ -841,8 +841,9 @@ int pp_logprobs(const void* logits, int64_t l_st, int dtype, int64_t rows, int64
  *   a' = scaling * (a cos w - b sin w),  b' = scaling * (b cos w + a sin w),
  *   w = 2 pi * position * turns[f] / 2^64,
  * position that of the row's token on axis axes[f]; the rest is copied.  turns (device) is each pair's
- * frequency, the fraction of a turn that one step is, times 2^64; with it the angle is exact for every 64-bit
- * position, negative ones (which turn back) among them.  axes (device; null: all 0) holds numbers below n_axes.
+ * frequency, the fraction of a turn that one step is, times 2^64; of that number the angle is exact for every 64-bit
+ * position, negative ones (which turn back) among them.  Sines and cosines are within 1e-7 (keys for 4 bits: 2e-16).
+ * axes (device; null: all 0) holds numbers below n_axes.
  */
 enum pp_pairs { PP_PAIRS_HALVES = 0, PP_PAIRS_NEIGHBOURS = 1 };
 enum pp_positions { PP_POS_I32 = 0, PP_POS_I64 = 1 };

@@ -42,10 +42,13 @@ class Rotary:
         a' = scaling * (a cos - b sin)        b' = scaling * (b cos + a sin)
 
     with ``scaling`` held in float32.  ``inv_freq`` holds rotary_dim / 2 numbers up to 2**58, by default
-    ``base ** (-2 f / rotary_dim)``; other spacings (stretched contexts) are given that way.  With several axes a token has a position on each:
-    ``sections`` says how many frequencies each axis turns, one axis after another, or ``axes`` names
-    the axis of every frequency (in turn, say).  Frequencies are kept as 64-bit fractions of a turn, so angles of
-    far positions are as exact as those of near ones; there is no table and no largest position.
+    ``base ** (-2 f / rotary_dim)``; other spacings (stretched contexts) are given that way.  With several axes a
+    token has a position on each: ``sections`` says how many frequencies each axis turns, one axis after
+    another, or ``axes`` names the axis of every frequency (in turn, say).
+
+    There is no table of positions, and any 64-bit position is taken.  A frequency is held to 2**-65 of a turn, so the
+    angle of a position is off by up to ``abs(position) * 2**-65`` turns, 2e-13 radians at 10**6.  Below 2**38
+    that is less than a sine in float32 is off by; at 2**62 it is most of a radian.
     """
 
     def __init__(self, head_dim, *, base=10000.0, rotary_dim=None, inv_freq=None, sections=None, axes=None,
@@ -123,9 +126,10 @@ def rotate(x, rotary, positions, *, out=None):
     """Rows ``x`` (tokens, heads, head_dim), float16, bfloat16 or float32, turned by ``positions``.
 
     ``positions`` int32 or int64: (tokens,) with one axis, (axes, tokens) with several; any numbers, negative ones
-    turn back.  Computed in float32 and rounded once to x's type.  ``out`` takes the result: x itself, or a tensor of its
-    shape and type in a storage of its own (another slice of the tensor that x is a slice of is refused); by default a new
-    one.  A backward pass that has saved ``out`` raises then, as after torch's own writes in place.
+    turn back.  Computed in float32, sines and cosines within 1e-7, and rounded once to x's type.  ``out`` takes
+    the result: x itself, or a tensor of its shape and type in a storage of its own (another slice of the tensor
+    that x is a slice of is refused); by default a new one.  A backward pass that has saved ``out`` raises then, as
+    after torch's own writes in place.
     """
     if x.dim() != 3 or x.dtype not in _ROWS:
         raise TypeError("x must be float16, bfloat16 or float32 (tokens, heads, head_dim)")

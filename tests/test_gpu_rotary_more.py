@@ -1,10 +1,14 @@
-"""rotate where the first tests of it do not look: how frequencies are given, tensors that a backward pass has saved."""
+"""rotate where the first tests of it do not look: how frequencies are given, the farthest positions, tensors that a
+backward pass has saved."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
 
-from polar_pack_amd.rotary import Rotary, rotate
+from polar_pack_amd.rotary import Rotary, _turn, rotate
 from serving import DEV
+from serving4 import PI, partners
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +53,17 @@ def test_frequencies_of_32_bits_are_what_they_are():
     want = rotate(x, Rotary(64, inv_freq=freqs.double()), pos)
     assert torch.equal(rotate(x, Rotary(64, inv_freq=freqs), pos), want)
     assert torch.equal(rotate(x, Rotary(64, inv_freq=freqs.numpy()), pos), want)
+
+
+@pytest.mark.parametrize("pos", [2 ** 62, 2 ** 63 - 1, -2 ** 63, 2 ** 55 + 3, -2 ** 47 - 1])
+def test_the_farthest_positions(pos):
+    """Of the fraction of a turn that is held, the angle keeps all its bits at any position: sines and cosines are off by no
+    more than near zero (the bound of the other tests; a 64-bit angle and its sine in the reference add 2^-51)."""
+    x = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(6))
+    freqs = [10000.0 ** (-f / 32) for f in range(32)]
+    rest = [Fraction(_turn(f) * pos % 2 ** 64, 2 ** 64) for f in freqs]
+    a = torch.tensor([float((t - 1 if 2 * t > 1 else t) * 2 * PI) for t in rest], dtype=torch.float64)
+    c, s, v = torch.cos(a), torch.sin(a), x.double()
+    want = torch.cat([v[..., :32] * c - v[..., 32:] * s, v[..., 32:] * c + v[..., :32] * s], 2)
+    got = rotate(x.to(DEV), Rotary(64), torch.tensor([pos], device=DEV)).cpu().double()
+    assert ((got - want).abs() <= (2.0 ** -22 + 2.0 ** -50) * partners(v, 64, "halves") + 2.0 ** -24 * want.abs()).all()
