@@ -810,12 +810,17 @@ int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_t table_ld,
  * A row that sees no key gives zeros and lse -inf.  q is (tokens, q_heads, head_dim) with strides q_st,
  * q_sh (PP_F16 or PP_BF16), out dense of the same type at a 16-byte boundary, lse null or (tokens,
  * q_heads) float32.  The workspace (pp_kv_attention_workspace_size bytes, 0: none) needs no initial values;
- * the counts (pp_kv_attention_counts_size bytes, 0: none) are zero on entry and left zero.
+ * the counts (pp_kv_attention_counts_size bytes, 0: none) are zero on entry and left zero.  These sizes do for any codes; with
+ * `codes` (pp_kv_codes) they are what a cache of these needs, which for 8 bits may be half as much.
  */
 int64_t pp_kv_attention_workspace_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
                                        int64_t batch, int64_t tokens, int64_t q_heads);
 int64_t pp_kv_attention_counts_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
                                     int64_t batch, int64_t tokens, int64_t q_heads);
+int64_t pp_kv_attention_codes_workspace_size(int64_t codes, int64_t heads, int64_t head_dim, int64_t block,
+                                             int64_t table_width, int64_t batch, int64_t tokens, int64_t q_heads);
+int64_t pp_kv_attention_codes_counts_size(int64_t codes, int64_t heads, int64_t head_dim, int64_t block,
+                                          int64_t table_width, int64_t batch, int64_t tokens, int64_t q_heads);
 int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                     int64_t tokens, const int32_t* table, int64_t table_ld, int64_t table_width,
                     const int32_t* lengths, const int32_t* cu, int64_t batch, int causal, int64_t window, float scale,

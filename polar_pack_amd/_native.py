@@ -153,6 +153,8 @@ EXPORTS = {
     "pp_kv_read": (i32, [vp, vp, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp]),
     "pp_kv_attention_workspace_size": (i64, [i64] * 7),
     "pp_kv_attention_counts_size": (i64, [i64] * 7),
+    "pp_kv_attention_codes_workspace_size": (i64, [i64] * 8),
+    "pp_kv_attention_codes_counts_size": (i64, [i64] * 8),
     "pp_kv_attention": (i32, [vp, vp, i64, i64, i64, i32, i64, vp, i64, i64, vp, vp, i64, i32, i64, C.c_float, vp, vp,
                               vp, i64, vp, i64, vp]),
     "pp_logprobs_workspace_size": (i64, [i64, i64, i64]),

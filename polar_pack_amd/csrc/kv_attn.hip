@@ -47,27 +47,35 @@ static AttnPlan attn_plan(int64_t heads, int64_t D, int64_t block, int64_t width
 
 using namespace pp;
 
-static bool attn_sizes(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
-                       int64_t q_heads, AttnPlan* P) {
-  if (heads <= 0 || D <= 0 || block <= 0 || width <= 0 || batch <= 0 || tokens <= 0 || q_heads < heads) return false;
-  // what either kind of codes needs
-  *P = attn_plan(heads, D, block, width, batch, tokens, q_heads, false);
-  const AttnPlan four = attn_plan(heads, D, block, width, batch, tokens, q_heads, true);
-  P->bytes = P->bytes > four.bytes ? P->bytes : four.bytes;
-  P->counts = P->counts > four.counts ? P->counts : four.counts;
-  return true;
+// What a call over codes of this kind needs; nothing where the sizes are none.
+static AttnPlan attn_sizes(int64_t heads, int64_t D, int64_t block, int64_t width, int64_t batch, int64_t tokens,
+                           int64_t q_heads, bool four) {
+  if (heads <= 0 || D <= 0 || block <= 0 || width <= 0 || batch <= 0 || tokens <= 0 || q_heads < heads) return AttnPlan{};
+  return attn_plan(heads, D, block, width, batch, tokens, q_heads, four);
+}
+
+extern "C" int64_t pp_kv_attention_codes_workspace_size(int64_t codes, int64_t heads, int64_t head_dim, int64_t block,
+                                                        int64_t table_width, int64_t batch, int64_t tokens, int64_t q_heads) {
+  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, codes == PP_KV_E2M1).bytes;
+}
+
+extern "C" int64_t pp_kv_attention_codes_counts_size(int64_t codes, int64_t heads, int64_t head_dim, int64_t block,
+                                                     int64_t table_width, int64_t batch, int64_t tokens, int64_t q_heads) {
+  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, codes == PP_KV_E2M1).counts;
 }
 
 extern "C" int64_t pp_kv_attention_workspace_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
                                                   int64_t batch, int64_t tokens, int64_t q_heads) {
-  AttnPlan P;
-  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, &P) ? P.bytes : 0;
+  const int64_t eight = attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, false).bytes;
+  const int64_t four = attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, true).bytes;
+  return eight > four ? eight : four;
 }
 
 extern "C" int64_t pp_kv_attention_counts_size(int64_t heads, int64_t head_dim, int64_t block, int64_t table_width,
                                                int64_t batch, int64_t tokens, int64_t q_heads) {
-  AttnPlan P;
-  return attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, &P) ? P.counts : 0;
+  const int64_t eight = attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, false).counts;
+  const int64_t four = attn_sizes(heads, head_dim, block, table_width, batch, tokens, q_heads, true).counts;
+  return eight > four ? eight : four;
 }
 
 extern "C" int pp_kv_attention(const pp_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads,

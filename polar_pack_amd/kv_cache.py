@@ -298,9 +298,9 @@ def kv_attention(q, cache, block_table, lengths, cu=None, *, causal=True, window
     with nat.on_device(dev):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty(n, heads, dtype=torch.float32, device=dev) if return_lse else None
-        shape = (dev.index, cache.heads, cache.head_dim, cache.block, call[2], call[5], n, heads)
-        size = nat.sized("pp_kv_attention_workspace_size", *shape)
-        n_counts = nat.sized("pp_kv_attention_counts_size", *shape)
+        shape = (dev.index, cache._abi.codes, cache.heads, cache.head_dim, cache.block, call[2], call[5], n, heads)
+        size = nat.sized("pp_kv_attention_codes_workspace_size", *shape)
+        n_counts = nat.sized("pp_kv_attention_codes_counts_size", *shape)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         counts, key = nat.zero_workspace(dev, n_counts)
         rc = nat.lib().pp_kv_attention(cache._ref, *at, heads, _VALUES[q.dtype], n,
