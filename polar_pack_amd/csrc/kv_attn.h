@@ -5,9 +5,12 @@
 
 namespace pp {
 
-// Weights are 2^(s - ref), s with log2 of vs in it, ref 14 below the largest s: up to 2^14 in fp16, the smallest that is
-// not flushed 2^-38 of the largest.  Past 2^24 floats are so far apart that the 14 would round to 16, whose 2^16 fp16
-// does not hold; ref is the largest s itself there.
+// Weights are 2^(s - ref), in 8 bits with log2 of vs in s, ref 14 below the largest s: up to 2^14 in fp16, so rounded to 11 bits,
+// or to 2^-39 of the largest where they are below 2^-28 of it (2^-37 of many rows, whose ref is up to 12 below and moves seldom);
+// what is below half of that is 0.  In 4 bits V's scales differ from group to group of a token's values, so they are
+// in V's operand and a weight is small by its score alone: n keys of tiny weights and values far above those of the largest
+// weights are off by up to n 2^-39 (2^-37) of the largest value, which the cache's documentation states.  Past 2^24
+// floats are so far apart that the 14 would round to 16, whose 2^16 fp16 does not hold; ref is the largest s itself there.
 constexpr float KV_P_LOG2 = 14.f;
 __device__ __forceinline__ float kv_ref(float top) {
   const float ref = top - KV_P_LOG2;

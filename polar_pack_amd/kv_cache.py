@@ -95,6 +95,13 @@ class KVCache4:
     token's codes depend on no other token.  NaN as each of a token's ``k_scale`` makes the token NaN for every row
     that sees it; scales of tokens before a sequence's length are otherwise as :func:`kv_append` writes them.  What lies past
     the lengths may hold anything.
+
+    Attention rounds a row's weights to fp16, by their scores alone: relative to the largest, to 11 bits or to 2**-37,
+    whichever is coarser.  So an output is off by up to 2**-11 of the weighted mean of its magnitudes, and by
+    2**-37 of the largest magnitude times the keys that the row sees.  The second part shows only where keys 19 nats and more
+    below the largest score hold values that are larger by a factor near 2**26 over their number; an 8-bit cache, whose
+    scales enter the weights, does not have it.
+
     :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.
     """
 
