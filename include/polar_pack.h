@@ -48,7 +48,7 @@ const char* pp_version(void);
 
 /* sizeof of the ABI structs, for binding checks: out[0] = sizeof(pp_quad_proj),
  * out[1] = sizeof(pp_quad_item), out[2] = sizeof(pp_quad_seg), out[3] = sizeof(pp_dual_proj),
- * out[4] = sizeof(pp_kv_cache).
+ * out[4] = sizeof(pp_kv_cache), out[5] = sizeof(pp_rotary).
  * Returns the number of values written. */
 int pp_abi_sizes(int64_t* out, int n);
 

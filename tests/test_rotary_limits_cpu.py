@@ -1,8 +1,10 @@
 """Numbers that a Rotary cannot hold are refused before any device is asked; those it can are held to their last bit."""
+import ctypes as C
 from fractions import Fraction
 
 import pytest
 
+from polar_pack_amd import _native as nat
 from polar_pack_amd.rotary import Rotary, _turn
 from serving4 import _pi
 
@@ -27,3 +29,9 @@ def test_fractions_of_a_turn(freq):
     turns = Fraction(freq) * (1 << 250) / (2 * _pi(250)) * (1 << 64)
     off = (turns - _turn(freq)) % (1 << 64)
     assert min(off, (1 << 64) - off) <= Fraction(1, 2) + Fraction(1, 4)
+
+
+def test_the_struct_is_as_long_as_the_library_has_it():
+    out = (C.c_int64 * 6)()
+    assert nat.lib().pp_abi_sizes(out, 6) == 6
+    assert out[5] == C.sizeof(nat.Rotary) and out[4] == C.sizeof(nat.KVCache)
