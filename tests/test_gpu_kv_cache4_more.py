@@ -1,4 +1,5 @@
-"""The 4-bit cache where the first tests of it do not look: turned keys that lie next to a border between two codes."""
+"""The 4-bit cache where the first tests of it do not look: turned keys that lie next to a border between two codes, and
+drafts that are written over."""
 import math
 from fractions import Fraction
 
@@ -8,6 +9,7 @@ import torch
 from polar_pack_amd.kv_cache import KVCache4, kv_read, kv_rotate_append
 from polar_pack_amd.rotary import Rotary
 from serving import DEV
+from serving4 import unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +61,33 @@ def test_turned_keys_beside_a_border():
     got = kv_read(cache, *at, dtype=torch.float32)[0][0, 0].tolist()
     assert got[31] == 6.0
     assert got[:len(cases)] == [up for _, _, up in cases]
+
+
+def test_drafts_that_were_refused_leave_nothing():
+    """Steps append five drafted tokens, of which some stay and the next step writes over the rest, not finite ones among
+    them: what lies below the length is byte for byte what one append of the tokens that stayed leaves."""
+    H, D, bs, n = 2, 64, 16, 60
+    g = torch.Generator().manual_seed(9)
+    k, v, q = (torch.randn(n, h, D, generator=g).half().to(DEV) for h in (H, H, 3))
+    r, table = Rotary(D), torch.tensor([[2, 0, 4, 1, 3]], dtype=torch.int32, device=DEV)
+    lengths = lambda m: torch.tensor([m], dtype=torch.int32, device=DEV)
+    cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device=DEV)
+    whole, steps = (KVCache4.zeros(5, H, D, block=bs, device=DEV) for _ in range(2))
+    want = kv_rotate_append(whole, q, k, v, r, table, lengths(n), cu(n))
+    at, i, turned = 0, 0, []
+    while at < n:
+        stay = min([3, 1, 5, 2, 4][i % 5], n - at)
+        kk, vv, qq = (torch.randn(5, h, D, generator=g).half().to(DEV) * 5 for h in (H, H, 3))
+        kk[:stay], vv[:stay], qq[:stay] = k[at:at + stay], v[at:at + stay], q[at:at + stay]
+        if stay < 5:
+            (kk if i % 2 else vv)[4, i % H, 7] = float("nan" if i % 3 else "inf")
+        turned.append(kv_rotate_append(steps, qq, kk, vv, r, table, lengths(at + 5), cu(5))[:stay])
+        at, i = at + stay, i + 1
+    assert torch.equal(torch.cat(turned), want)
+    for p in range(5):
+        page, seen = int(table[0, p]), min(max(n - p * bs, 0), bs)
+        for name, axis in (("k", 1), ("k_scale", 1), ("v_scale", 2)):
+            a, b = (getattr(c, name).view(torch.uint8)[page].narrow(axis, 0, seen) for c in (steps, whole))
+            assert torch.equal(a, b), (p, name)
+        a, b = (unpack(c.v[page].cpu())[..., :seen] for c in (steps, whole))
+        assert torch.equal(a, b), p

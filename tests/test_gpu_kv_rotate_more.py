@@ -133,3 +133,47 @@ def test_append_of_many_axes(n_axes, pairs):
             read = eight.k[page, :, p % bs].cpu().double() * s
             assert ((read - turned[i]).abs() <= 0.5 * s * (1 + 2.0 ** -20) + off[i]).all()
             i += 1
+
+
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("H,D,bs", [(2, 128, 64), (1, 64, 16), (1, 256, 128)])
+def test_codes_that_are_rounded_again(H, D, bs, kind):
+    """Where a page's scale grew, its earlier tokens' codes are round(code * (old / new)) of the scales before and after, to
+    the bit; where it did not, they are as they were; and the new scale is what the turned keys ask for, to their own error."""
+    lens, news = [bs - 1, 2 * bs - 3, bs + 9, 3 * bs - 5], [2, 7, 5, bs]
+    g = torch.Generator().manual_seed(D)
+    pages = sum(-(-n // bs) for n in lens)
+    parts, table = random_cache(pages, H, bs, D, kind, g), tables(lens, bs, pages, g)
+    k, v = (torch.randn(sum(news), H, D, generator=g).half() for _ in range(2))
+    k[2:9] *= 0.02                                               # a page whose scale stays
+    cache = device_cache(parts)
+    freqs = [10000.0 ** (-2 * f / D) for f in range(D // 2)]
+    at = (table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), offsets(news).to(DEV))
+    kv_rotate_append(cache, None, k.to(DEV), v.to(DEV), Rotary(D), *at)
+    own = [p for L, n in zip(lens, news) for p in range(L - n, L)]
+    turned = turn(k.double(), D, "halves", freqs, [0] * (D // 2), [own])
+    pair = partners(k.double(), D, "halves")
+    now, was = cache.k_scale.cpu(), parts[2]
+    qmax = 127.0 if kind == torch.int8 else 448.0
+    grew = kept = i = 0
+    for b, (L, n) in enumerate(zip(lens, news)):
+        first = (L - n) // bs                                    # the page that holds earlier tokens
+        page, held, new = int(table[b, first]), (L - n) % bs, min(n, bs - (L - n) % bs)
+        top = turned[i:i + new].abs().amax((0, 2))
+        off = pair[i:i + new].amax((0, 2)) * 2.0 ** -22
+        i += n
+        if held == 0:
+            continue
+        for h in range(H):
+            need = torch.clamp(top[h] / qmax, min=float(was[page, h]))
+            assert abs(float(now[page, h]) - float(need)) <= float(off[h]) / qmax + 2.0 ** -23 * float(need)
+            old = parts[0][page, h, :held]
+            if now[page, h] > was[page, h]:
+                x = old.float() * (was[page, h] / now[page, h])
+                old = (x.round() if kind == torch.int8 else x).to(kind)
+                grew += 1
+            else:
+                assert now[page, h] == was[page, h]
+                kept += 1
+            assert torch.equal(raw(cache.k[page, h, :held]).cpu(), raw(old))
+    assert grew and kept
