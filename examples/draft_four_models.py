@@ -32,6 +32,7 @@ class Drafting(Models):
         self.drafts = drafts
         self.text = torch.zeros(MODELS, context + drafts + 1, dtype=torch.int64, device=device)
         self.size = torch.zeros(MODELS, dtype=torch.int64, device=device)
+        self.context, self.most = context, 0
 
     def forward(self, tokens, lengths):
         """Logits (models, n, VOCAB) after each of ``tokens`` (models, n), the last of ``lengths`` (models,) each."""
@@ -47,7 +48,10 @@ class Drafting(Models):
     def begin(self, prompt):
         """Take in all of ``prompt`` (models, n) but its last token."""
         n = prompt.shape[1]
+        if n > self.context:
+            raise ValueError(f"a prompt of {n} tokens in a context of {self.context}")
         self.text[:, :n] = prompt
+        self.most = n
         self.size.fill_(n)
         self.forward(prompt[:, :-1], self.size - 1)
 
@@ -62,7 +66,11 @@ class Drafting(Models):
         return last, tokens, counts.int()
 
     def step(self, uniforms, temperature=0.7):
-        """One step with ``uniforms`` (models, drafts + 1): what was drafted and what became of it."""
+        """One step with ``uniforms`` (models, drafts + 1): what was drafted and what became of it.  How long the texts are
+        only the device knows, so a step is refused where they could be longer than the context, all drafts kept."""
+        if self.most > self.context:
+            raise ValueError(f"texts of up to {self.most} tokens in a context of {self.context}")
+        self.most += self.drafts + 1
         last, tokens, counts = self.look_up()
         logits = self.forward(torch.cat([last, tokens], 1), self.size + self.drafts)
         target = torch.softmax(logits.float() / temperature, 2)
