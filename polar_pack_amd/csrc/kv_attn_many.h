@@ -18,11 +18,14 @@
 // 32,192: 166 us, 0.82.  Measured on the way (prompts / piece): wavefronts of 64 rows, one a SIMD 395 / 442 us (registers spilled),
 // 8 of 32 rows 142 / 182, a barrier apart 144 / 167, heavy row tiles first and priority 103 / 164.
 // 192 and 256 values a head: sums and queries of 32 rows take 144 and 192 registers, so 4 wavefronts, one a SIMD,
-// whose products wait for their weights; at 256 28 bytes a lane spill.  The same prompts with 12 query and 4 key heads of 192
+// whose products wait for their weights; at 256 28-32 bytes a lane spill (140-152 in pages of 16).  The same prompts with 12 query and 4 key heads of 192
 // 175 us, 0.44 PFLOP/s (a piece 272, 0.56), with 16 and 1 of 256 278, 0.50 (424, 0.64).
 //
 // 4 bits (PP_KV_E2M1): codes become halves with their scales on the way into LDS, where everything is as in 8 bits; the products
-// and weights bound it as there.  509 tokens behind 32,192: 159 us, 0.85 PFLOP/s (8 bits 161).
+// and weights bound it as there.  509 tokens behind 32,192: 159 us, 0.85 PFLOP/s (8 bits 161).  At 256 values a head a thread
+// stages four pieces of V, each with 16 bytes of scales, and 148-152 bytes a lane spill (220-224 in pages of 16); at 192 nothing does.
+// In turn with 8 bits, us: four prompts of 2048 with 16 query and 2 key heads of 128 93 / 99, 12 and 4 of 192 166 / 169, 16 and 1
+// of 256 272 / 254 (0.51 PFLOP/s; in pages of 16 383 / 300); 509 behind 32,192 149 / 161, 252 / 263 and 418 / 399 (0.65).
 #pragma once
 
 #include "kv_attn.h"

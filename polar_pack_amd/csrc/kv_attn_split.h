@@ -42,6 +42,9 @@ namespace pp {
 // as the loads, and a SIMD issues an instruction of one wavefront every 8 clocks, of two every 4 to 5.  64 sequences of
 // 77-8190 tokens and 8 key heads (297 MB) 64 us, 4.6 TB/s, with one workgroup of two tiles a CU 73; loads alone take
 // 62.  4 sequences of 200-262 k and 2 (263 MB) 57 us: there two workgroups a CU would leave twice the parts to join (61).
+// Wider heads, in turn with 8 bits, us: 64 of 77-8190 with 4 key heads of 192 60 / 88 (3.8 TB/s), of 256 72 / 117 (4.3); 4 of 100-131 k
+// with 2 of 192 50 / 76, of 256 59 / 100 (4.3).  In tiles of 32 rows the registers are full: 24 sequences of 500-8000 and 5 drafted
+// tokens with 8 key heads of 128 54 / 61, 4 of 192 49 / 52, 4 of 256 84 / 76, where 208-212 bytes a lane spill; elsewhere nothing does.
 // The scaled products that take 4-bit codes as they are were no way: against queries split over three e4m3 terms they are off
 // by 2^-15 of the sum of magnitudes, where float32 sums are by 2^-24.
 template <int CODES, typename IO, int D, int RT, int NP>

@@ -7,7 +7,7 @@
 // between: a step of 4 bits is wide, and a rounding before it would move one value in some 10^7 by a whole step.
 //
 // What bounds it: instructions beside memory.  16 ragged prompts (14,752 tokens), 8 key heads and 32 query heads of 128
-// in bf16, 305 MB: 78 us, 3.9 TB/s with the vector units 49 % busy; the queries' rows alone would take 44, the keys and
+// in bf16, 305 MB: 77 us, 4.0 TB/s with the vector units 49 % busy; the queries' rows alone would take 44, the keys and
 // values alone 31 (not turned 18).  The keys' sines in 64 bits, once for four heads, and their rounding to odd are a third of the
 // instructions.  64 single tokens 7.9 us, latency.  Reading back 17 us (58 MB written, 4.7 TB/s).
 #include "kv_cache4.h"

@@ -1,8 +1,8 @@
 // Queries and keys turned by their positions, keys and values written to the cache, in one launch: 8 bits and the
 // entry point.
 //
-// What bounds it: the queries' way through memory, and instructions (61 % busy).  4 prompts of 2048 tokens, 16 query and
-// 2 key heads of 128 in fp16, 81 MB: 20 us, 4.0 TB/s (34 with heads one after another and appends before all queries);
+// What bounds it: the queries' way through memory, and instructions (63 % busy).  4 prompts of 2048 tokens, 16 query and
+// 2 key heads of 128 in fp16, 81 MB: 21 us, 3.9 TB/s (34 with heads one after another and appends before all queries);
 // single tokens of 4 sequences 7.8 us, as an append without rotation (7.4): the chain of lengths, pages, values and old scale.
 #include "kv_cache4.h"
 #include "rotate_keys.h"
