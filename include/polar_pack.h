@@ -807,8 +807,9 @@ int pp_kv_read(const pp_kv_cache* cache, const int32_t* table, int64_t table_ld,
  * (p - window, p] (causal; window 0: of [0, p]), or all of [0, lengths[b]) (causal 0); causal or not, a row
  * with p < 0, where a sequence has more of the call's tokens than lengths[b], sees none:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
- * Weights are rounded to fp16 for the product with the values: relative to a row's largest, to 11 bits or (4 bits, whose
- * scales are not in the weights) to 2^-37, whichever is coarser, so that there n keys add up to n 2^-37 of the largest |v|.
+ * Weights, in 8 bits times their page's v scale, are rounded to fp16 for the product with the values (4 bits) or codes: relative to a
+ * row's largest, to 11 bits or to 2^-37, whichever is coarser, so n keys of tiny weights add up to n 2^-37 of the largest |v| (8
+ * bits: of the largest product times 127 or 448).
  * A row that sees no key gives zeros and lse -inf.  q is (tokens, q_heads, head_dim) with strides q_st,
  * q_sh (PP_F16 or PP_BF16), out dense of the same type at a 16-byte boundary, lse null or (tokens,
  * q_heads) float32.  The workspace (pp_kv_attention_workspace_size bytes, 0: none) needs no initial values;

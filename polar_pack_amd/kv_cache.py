@@ -99,8 +99,8 @@ class KVCache4:
     Attention rounds a row's weights to fp16, by their scores alone: relative to the largest, to 11 bits or to 2**-37,
     whichever is coarser.  So an output is off by up to 2**-11 of the weighted mean of its magnitudes, and by
     2**-37 of the largest magnitude times the keys that the row sees.  The second part shows only where keys 19 nats and more
-    below the largest score hold values that are larger by a factor near 2**26 over their number; an 8-bit cache, whose
-    scales enter the weights, does not have it.
+    below the largest score hold values that are larger by a factor near 2**26 over their number.  (In an 8-bit cache a
+    page's scale is in its weights, and there it is 2**-37 of the largest weight times scale, times qmax.)
 
     :meth:`zeros` makes a cache; the constructor takes tensors that a program holds already.
     """
